@@ -1,0 +1,79 @@
+// 8-bit floats in blocks of 128 with one power-of-two scale each: the format, its rounding, and the
+// tensor-core instruction that takes the scales.
+//
+// A block holds q in e4m3 (or e5m2) and a scale byte e (biased by 127): its values are q * 2^(e - 127).
+// e is the smallest with which the block's largest magnitude is at most fmax = 448 (57344): both are
+// 1.75 * 2^n, so e follows from the exponent of that magnitude, plus one where its mantissa is above 0.75.
+// With powers of two scaling is exact in both directions, the one rounding of a value is that to its 3 (2)
+// mantissa bits, and the tensor cores multiply by the scales themselves (kind::mxf8f6f4.block_scale), at
+// their full 8-bit rate. Factors with a mantissa would have to be applied to every partial sum of 128 in
+// registers; what they would buy is less than one bit of range at the lower end of a block.
+//   * a block of zeros has the scale 1 (e = 127);
+//   * e is kept in [1, 254], normal powers of two (magnitudes below 2^-118 lose range, not scale);
+//   * a block with a NaN or an infinity is NaN throughout (q = 0x7f, e = 127): a product shows it, where
+//     saturated values would hide it.
+//
+// Scales of a matrix [rows, K] lie as words [ceil(K / 512)][rows]: byte kb % 4 of word (kb / 4, row) is the
+// scale of columns 128 kb .. 128 kb + 127 of that row. 128 x 128 blocks repeat theirs for every row. So a
+// warp reads the words of 32 rows as one line, a word is what the tensor memory holds for a row and
+// four blocks, and no row count needs padding.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "../common/ptx.cuh"
+
+namespace lb {
+
+constexpr int kScaleBlock = 128;
+constexpr uint32_t kScaleOne = 127u;
+
+// Scale byte of a block whose largest magnitude has the bf16 bits `a` (finite).
+template <int E5M2>
+__device__ __forceinline__ uint32_t block_scale_byte(uint32_t a) {
+  if (a == 0u) return kScaleOne;
+  const int e = int(a >> 7) - (E5M2 ? 15 : 8) + ((a & 0x7fu) > 0x60u ? 1 : 0);
+  return uint32_t(min(max(e, 1), 254));
+}
+__device__ __forceinline__ bool block_is_finite(uint32_t a) { return a < 0x7f80u; }
+// 2^(127 - e): what a value is multiplied by before it is rounded.
+__device__ __forceinline__ float block_inverse(uint32_t e) { return __uint_as_float((254u - e) << 23); }
+
+// D[tmem] (+)= (A[smem] * scales) * (B[smem] * scales), 8-bit floats, 32 elements of depth. The scale
+// operands are tensor-memory addresses: row r's word lies in lane r % 32 (of every quarter of the lanes),
+// column r / 32; the instruction descriptor says which of its bytes applies.
+__device__ __forceinline__ void umma_block(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
+                                           uint32_t idesc, uint32_t tmem_sa, uint32_t tmem_sb,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %6, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n"
+      "}\n"
+      :
+      : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor of kind::mxf8f6f4: operand formats 0 = e4m3, 1 = e5m2, both K-major; scales are
+// powers of two (bit 23), byte `sf` of their words.
+__device__ __forceinline__ uint32_t umma_idesc_block(int M, int N, int a_e5m2, int b_e5m2, int sf) {
+  return (uint32_t(sf) << 4)             // which byte of B's words
+         | (uint32_t(a_e5m2) << 7)       // A format
+         | (uint32_t(b_e5m2) << 10)      // B format
+         | (uint32_t(N >> 3) << 17)      // N / 8
+         | (1u << 23)                    // scale format: exponents
+         | (uint32_t(M >> 7) << 27)      // M / 128
+         | (uint32_t(sf) << 29);         // which byte of A's words
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+
+}  // namespace lb

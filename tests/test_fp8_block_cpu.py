@@ -1,0 +1,262 @@
+"""Block-scaled 8-bit operators on the CPU: the format, the eager arithmetic that the GPU kernels are held to,
+and what is refused."""
+import math
+
+import pytest
+import torch
+
+from lset_b200.ops import fp8_block as fb
+
+
+def _by_hand(block, e5m2):
+    """A block's values after the cast, one by one in Python floats (64 bits)."""
+    top = max(abs(v) for v in block)
+    if not math.isfinite(top) or any(math.isnan(v) for v in block):
+        return [math.nan] * len(block)
+    fmax, bits, low = (57344.0, 2, -14) if e5m2 else (448.0, 3, -6)
+    e = -126
+    while top > fmax * 2.0 ** e:
+        e += 1
+    if top == 0:
+        e = 0
+    out = []
+    for v in block:
+        y = v / 2.0 ** e
+        step = 2.0 ** (max(math.frexp(y)[1] - 1, low) - bits)
+        out.append(round(y / step) * step * 2.0 ** e)     # Python rounds halves to even
+    return out
+
+
+def _same(a, b):
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(nan=0.0), b.nan_to_num(nan=0.0))
+
+
+SPECIAL = [0.0, 448.0, 449.0, 450.0, -448.0, 1e-30, 2.0 ** -133, 3.3e38, 2.0 ** -126, 57344.0, 57600.0, 1.75, 1.7578125]
+
+
+@pytest.mark.parametrize("e5m2", [False, True])
+@pytest.mark.parametrize("R,C", [(1, 1), (3, 130), (129, 24), (128, 128), (257, 131)])
+def test_values_of_every_kind_of_block(R, C, e5m2):
+    g = torch.Generator().manual_seed(R * C)
+    x = (torch.randn(R, C, generator=g) * torch.exp(4 * torch.randn(R, C, generator=g))).to(torch.bfloat16)
+    for i, v in enumerate(SPECIAL):
+        x[(i * 5) % R, (i * 37) % C] = v
+    if R > 2:
+        x[2] = 0
+    xl = x.double().tolist()
+    rows = torch.tensor([sum((_by_hand(r[c:c + 128], e5m2) for c in range(0, C, 128)), []) for r in xl])
+    cols = torch.tensor([sum((_by_hand(r[c:c + 128], e5m2) for c in range(0, R, 128)), [])
+                         for r in x.double().t().tolist()])
+    q, q_t = fb.quantize_fp8_block(x, e5m2=e5m2, want_t=True)
+    assert q.shape == (R, C) and q_t.shape == (C, R)
+    assert _same(q.dequantize(), rows.float()) and _same(q_t.dequantize(), cols.float())
+    t, t_t = fb.quantize_fp8_block(x, tile=True, e5m2=e5m2, want_t=True)
+    tiles = torch.zeros(R, C)
+    for r in range(0, R, 128):
+        for c in range(0, C, 128):
+            part = x[r:r + 128, c:c + 128].double()
+            tiles[r:r + 128, c:c + 128] = torch.tensor(_by_hand(part.flatten().tolist(), e5m2)).view(part.shape)
+    assert _same(t.dequantize(), tiles) and _same(t_t.dequantize(), tiles.t())
+    for v in (q, q_t, t, t_t):
+        v.check("q")
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_a_block_that_is_not_finite_is_nan_and_no_other(bad):
+    x = torch.ones(5, 300, dtype=torch.bfloat16)
+    x[1, 140] = bad
+    q, q_t = fb.quantize_fp8_block(x, want_t=True)
+    want = torch.zeros(5, 300, dtype=torch.bool)
+    want[1, 128:256] = True
+    assert torch.equal(torch.isnan(q.dequantize()), want)
+    want = torch.zeros(300, 5, dtype=torch.bool)
+    want[140] = True
+    assert torch.equal(torch.isnan(q_t.dequantize()), want)
+    t, _ = fb.quantize_fp8_block(x, tile=True)
+    assert torch.isnan(t.dequantize()[:, 128:256]).all() and not torch.isnan(t.dequantize()[:, :128]).any()
+
+
+def test_products_and_accumulation():
+    torch.manual_seed(1)
+    a, _ = fb.quantize_fp8_block(torch.randn(7, 200))
+    b, _ = fb.quantize_fp8_block(torch.randn(24, 200), tile=True, e5m2=True)
+    ref = a.dequantize().double() @ b.dequantize().double().t()
+    bound = 200 * 2.0 ** -23 * (a.dequantize().abs() @ b.dequantize().abs().t())
+    c = fb.matmul_fp8_block(a, b, out_dtype=torch.float32)
+    assert ((c - ref).abs() <= bound).all()
+    out = torch.ones(7, 24)
+    assert fb.matmul_fp8_block(a, b, out=out, accumulate=True) is out
+    assert ((out - 1 - ref).abs() <= bound + 2.0 ** -23 * (1 + ref.abs())).all()
+    bias = torch.randn(24)
+    y = fb.matmul_fp8_block(a, b, bias=bias)
+    assert y.dtype == torch.bfloat16
+    want = ref + bias.bfloat16().double()
+    assert ((y - want).abs() <= 2.0 ** -8 * want.abs() + 2 * bound + 1e-6).all()
+
+
+def test_linear_gradients_are_products_of_the_cast_operands():
+    torch.manual_seed(2)
+    x = torch.randn(3, 50, 136, requires_grad=True)
+    w, b = torch.randn(72, 136, requires_grad=True), torch.randn(72, requires_grad=True)
+    y = fb.linear_fp8_block(x, w, b)
+    dy = torch.randn_like(y)
+    y.backward(dy)
+    x2, d2 = x.detach().view(150, 136), dy.view(150, 72)
+    (xq, xt), (wq, _) = fb.quantize_fp8_block(x2, want_t=True), fb.quantize_fp8_block(w.detach(), tile=True)
+    dq, dt = fb.quantize_fp8_block(d2, want_t=True)
+    close = lambda got, a, c: torch.allclose(got, a @ c, rtol=1e-5, atol=1e-4)  # noqa: E731
+    assert y.dtype == torch.float32 and y.shape == (3, 50, 72)
+    assert close(y.detach().view(150, 72) - b.detach().bfloat16().float(), xq.dequantize(), wq.dequantize().t())
+    assert close(x.grad.view(150, 136), dq.dequantize(), wq.dequantize())
+    assert close(w.grad, dt.dequantize(), xt.dequantize().t())
+    assert torch.allclose(b.grad, d2.sum(0), atol=1e-4)
+    # the same values from a kept weight
+    with torch.no_grad():
+        assert torch.equal(fb.linear_fp8_block(x, wq, b), y)
+
+
+def test_refusals():
+    x = torch.randn(4, 64)
+    w = torch.randn(32, 64)
+    wq, _ = fb.quantize_fp8_block(w, tile=True)
+    xq, _ = fb.quantize_fp8_block(x)
+    with pytest.raises(ValueError, match="2-D"):
+        fb.quantize_fp8_block(torch.randn(2, 3, 64))
+    with pytest.raises(ValueError, match="floating"):
+        fb.quantize_fp8_block(torch.ones(4, 64, dtype=torch.int32))
+    with pytest.raises(ValueError, match="contraction"):
+        fb.matmul_fp8_block(xq, fb.quantize_fp8_block(torch.randn(32, 128))[0])
+    with pytest.raises(ValueError, match="out has to be"):
+        fb.matmul_fp8_block(xq, wq, out=torch.empty(4, 31))
+    with pytest.raises(ValueError, match="out has to be"):
+        fb.matmul_fp8_block(xq, wq, out=torch.empty(32, 4).t())
+    with pytest.raises(TypeError, match="bf16 or fp32"):
+        fb.matmul_fp8_block(xq, wq, out_dtype=torch.float16)
+    with pytest.raises(ValueError, match="accumulate"):
+        fb.matmul_fp8_block(xq, wq, accumulate=True)
+    with pytest.raises(ValueError, match="accumulate"):
+        fb.matmul_fp8_block(xq, wq, out=torch.zeros(4, 32, dtype=torch.bfloat16), accumulate=True)
+    with pytest.raises(ValueError, match="bias"):
+        fb.matmul_fp8_block(xq, wq, bias=torch.zeros(31))
+    with pytest.raises(ValueError, match="features"):
+        fb.linear_fp8_block(x, torch.randn(32, 63))
+    with pytest.raises(ValueError, match="without gradients"):
+        fb.linear_fp8_block(x.requires_grad_(), wq)
+    for broken in (fb.Fp8BlockTensor(wq.data, 640, wq.scales), fb.Fp8BlockTensor(wq.data, 64, wq.scales[:, :31]),
+                   fb.Fp8BlockTensor(wq.data.t(), 32, wq.scales), fb.Fp8BlockTensor(wq.data[:, :60], 64, wq.scales)):
+        with pytest.raises(ValueError):
+            fb.matmul_fp8_block(xq, broken)
+    with pytest.raises(TypeError):
+        fb.matmul_fp8_block(xq, fb.Fp8BlockTensor(wq.data.float(), 64, wq.scales))
+
+
+def test_empty_matrices():
+    e, e_t = fb.quantize_fp8_block(torch.empty(0, 64), want_t=True)
+    assert e.shape == (0, 64) and e_t.shape == (64, 0)
+    w, _ = fb.quantize_fp8_block(torch.randn(32, 64), tile=True)
+    assert fb.matmul_fp8_block(e, w).shape == (0, 32)
+    assert not fb.matmul_fp8_block(e_t, e_t).any()
+
+
+def test_linear_gradient_against_differences():
+    """On values that the format holds exactly (small whole numbers) the layer is linear, and so is a difference of
+    its outputs: both sides are whole numbers below 2^24, and equal."""
+    g = torch.Generator().manual_seed(3)
+    whole = lambda *s: torch.randint(-4, 5, s, generator=g).float()  # noqa: E731
+    x, w, dy = whole(140, 256).requires_grad_(), whole(16, 256).requires_grad_(), whole(140, 16)
+    fb.linear_fp8_block(x, w).backward(dy)
+    with torch.no_grad():
+        f = lambda a, b: (fb.linear_fp8_block(a, b).double() * dy).sum()  # noqa: E731
+        d = whole(140, 256)
+        assert f(x + d, w) - f(x, w) == (x.grad.double() * d).sum()
+        d = whole(16, 256)
+        assert f(x, w + d) - f(x, w) == (w.grad.double() * d).sum()
+
+
+def _mlp_reference(x, wg, wu, wd, kind, dy):
+    """The gated block by its formulas in 64 bits, from the cast values of its operands."""
+    r = lambda v, rows, cols: _cast_double(v, rows, cols)  # noqa: E731
+    bf = lambda v: v.to(torch.bfloat16).double()  # noqa: E731
+    xv, gv, uv, dv = r(x, 1, 128), r(wg, 128, 128), r(wu, 128, 128), r(wd, 128, 128)
+    g, u = bf(xv @ gv.t()).requires_grad_(), bf(xv @ uv.t()).requires_grad_()
+    act = torch.nn.functional.silu(g) if kind == "swiglu" else torch.nn.functional.gelu(g, approximate="tanh")
+    h = act * u
+    hb = bf(h.detach())
+    y = r(hb, 1, 128) @ dv.t()
+    dh = bf(r(dy, 1, 128) @ dv)
+    dg, du = (bf(t) for t in torch.autograd.grad(h, (g, u), dh))
+    dgu, wgu = torch.cat([dg, du], 1), torch.cat([gv, uv])
+    dw = r(dgu, 128, 1).t() @ r(x, 128, 1)
+    return y, r(dgu, 1, 128) @ wgu, dw[:g.shape[1]], dw[g.shape[1]:], r(dy, 128, 1).t() @ r(hb, 128, 1)
+
+
+def _cast_double(v, rows, cols):
+    """bf16 values in blocks of 1 x 128 (rows = 1), 128 x 1 or 128 x 128, as the (separately tested) cast has them."""
+    v = v.detach().to(torch.bfloat16)
+    if rows == 1:
+        return fb.quantize_fp8_block(v)[0].dequantize().double()
+    if cols == 1:
+        return fb.quantize_fp8_block(v, want=False, want_t=True)[1].dequantize().t().double()
+    return fb.quantize_fp8_block(v, tile=True)[0].dequantize().double()
+
+
+def _norm_off(a, b):
+    return float((a.double() - b).norm() / b.norm())
+
+
+@pytest.mark.parametrize("kind", ["swiglu", "geglu"])
+@pytest.mark.parametrize("T,H,I", [(1, 64, 128), (37, 136, 256), (130, 72, 384)])
+def test_gated_mlp_forward_and_gradients(T, H, I, kind):
+    g = torch.Generator().manual_seed(T + I)
+    n = lambda *s, scale=1.0: (torch.randn(*s, generator=g) * scale).to(torch.bfloat16)  # noqa: E731
+    x, dy = n(T, H), n(T, H)
+    wg, wu, wd = n(I, H, scale=H ** -0.5), n(I, H, scale=H ** -0.5), n(H, I, scale=I ** -0.5)
+    want = _mlp_reference(x, wg, wu, wd, kind, dy)
+    x.requires_grad_()
+    fused, wd = torch.cat([wg, wu]).requires_grad_(), wd.requires_grad_()
+    wg, wu = wg.requires_grad_(), wu.requires_grad_()
+    y = fb.gated_mlp_fp8_block(x, wg, wu, wd, kind)
+    got = [y.detach(), *torch.autograd.grad(y, (x, wg, wu, wd), dy)]
+    # outputs are rounded to bf16 (2^-8 of a value at most); a bf16 value in between that falls to the other side of
+    # a rounding in 32 bits moves by 2^-7 of itself, and its 8-bit form by up to 2^-3: rare, below 2^-7 of a norm
+    for a, b in zip(got, want):
+        assert a.dtype == torch.bfloat16 and _norm_off(a, b) < 2.0 ** -6
+    y2 = fb.gated_mlp_fp8_block(x, fused, None, wd, kind)
+    gf = torch.autograd.grad(y2, (x, fused, wd), dy)
+    assert torch.equal(y2, y) and torch.equal(gf[0], got[1])
+    assert torch.equal(gf[1], torch.cat([got[2], got[3]])) and torch.equal(gf[2], got[4])
+    with torch.no_grad():
+        kept = [fb.quantize_fp8_block(w, tile=True)[0] for w in (fused, wd)]
+        assert torch.equal(fb.gated_mlp_fp8_block(x, kept[0], None, kept[1], kind), y)
+
+
+def test_gated_mlp_gradients_of_some_inputs_only():
+    g = torch.Generator().manual_seed(5)
+    mk = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16)  # noqa: E731
+    x, wg, wu, wd, dy = mk(2, 9, 64), mk(128, 64), mk(128, 64), mk(64, 128), mk(2, 9, 64)
+    leaves = [x, wg, wu, wd]
+    for t in leaves:
+        t.requires_grad_()
+    full = torch.autograd.grad(fb.gated_mlp_fp8_block(*leaves), leaves, dy)
+    for i in range(4):
+        for t in leaves:
+            t.requires_grad_(t is leaves[i])
+        (one,) = torch.autograd.grad(fb.gated_mlp_fp8_block(*leaves), (leaves[i],), dy)
+        assert one.shape == leaves[i].shape and torch.equal(one, full[i])
+
+
+def test_gated_mlp_refusals():
+    x, wg, wd = torch.randn(3, 64), torch.randn(256, 64), torch.randn(64, 128)
+    with pytest.raises(ValueError, match="activation"):
+        fb.gated_mlp_fp8_block(x, wg, None, wd, "relu")
+    with pytest.raises(ValueError, match="multiple of 128"):
+        fb.gated_mlp_fp8_block(x, torch.randn(128, 64), None, torch.randn(64, 64))
+    with pytest.raises(ValueError, match="do not fit"):
+        fb.gated_mlp_fp8_block(x, wg, wg, wd)
+    with pytest.raises(ValueError, match="features"):
+        fb.gated_mlp_fp8_block(torch.randn(3, 65), wg, None, wd)
+    q = [fb.quantize_fp8_block(w, tile=True)[0] for w in (wg, wd)]
+    with pytest.raises(ValueError, match="8-bit weights"):
+        fb.gated_mlp_fp8_block(x, q[0], None, wd)
+    with pytest.raises(ValueError, match="without gradients"):
+        fb.gated_mlp_fp8_block(x.requires_grad_(), q[0], None, q[1])

@@ -1,0 +1,271 @@
+"""Block-scaled 8-bit operators on the GPU: the casts' bytes against the eager ones, products against 64-bit
+sums of the values that the operands stand for, layers against their definition."""
+import pytest
+import torch
+
+from lset_b200.ops import _native as nv
+from lset_b200.ops import fp8_block as fb
+
+pytestmark = pytest.mark.gpu
+
+
+def _rand(*shape, seed=0, spread=2.0):
+    g = torch.Generator("cuda").manual_seed(seed + sum(shape))
+    x = torch.randn(*shape, generator=g, device="cuda")
+    return (x * torch.exp(spread * torch.randn(*shape, generator=g, device="cuda"))).to(torch.bfloat16)
+
+
+def _same_bytes(got, want):
+    assert got.shape == want.shape and got.e5m2 == want.e5m2
+    assert torch.equal(got.data[:, :got.cols].cpu(), want.data[:, :want.cols])
+    assert torch.equal(got.scales.cpu(), want.scales)
+
+
+def _check_product(c, a, b, bias=None, base=None):
+    """Errors of a product: half a step of the output's type, and of the fp32 sums at most 2^-22 of the summed
+    magnitudes for each of the K / 32 instructions (a sum cut to 24 bits is off by 2^-23 of itself) and two more
+    for the products inside one."""
+    A, B = a.dequantize().double(), b.dequantize().double()
+    ref = A @ B.t()
+    if bias is not None:
+        ref = ref + bias.double()
+    if base is not None:
+        ref = ref + base.double()
+    sums = (a.cols // 32 + 3) * 2.0 ** -22 * (A.abs() @ B.abs().t())
+    half = 2.0 ** -8 if c.dtype == torch.bfloat16 else 2.0 ** -23
+    assert ((c.double() - ref).abs() <= half * ref.abs() + sums).all(), \
+        float(((c.double() - ref).abs() - half * ref.abs() - sums).max())
+
+
+@pytest.mark.parametrize("R,C", [(1, 8), (3, 136), (128, 128), (129, 520), (300, 264), (1000, 1032), (7, 4096)])
+@pytest.mark.parametrize("tile", [False, True])
+@pytest.mark.parametrize("e5m2", [False, True])
+def test_cast_has_the_bytes_of_the_eager_one(R, C, tile, e5m2):
+    x = _rand(R, C)
+    x[R // 2] = 0
+    x[0, 0], x[R - 1, C - 1] = 448.0, 2.0 ** -133
+    if R > 2:
+        x[1, C // 2], x[2, 1] = float("inf"), float("nan")
+    q, q_t = fb.quantize_fp8_block(x, tile=tile, e5m2=e5m2, want_t=True)
+    e, e_t = fb.quantize_fp8_block(x.cpu(), tile=tile, e5m2=e5m2, want_t=True)
+    _same_bytes(q, e)
+    _same_bytes(q_t, e_t)
+    only, none = fb.quantize_fp8_block(x, tile=tile, e5m2=e5m2)
+    assert none is None and torch.equal(only.data[:, :C], q.data[:, :C])
+    none, only = fb.quantize_fp8_block(x, tile=tile, e5m2=e5m2, want=False, want_t=True)
+    assert none is None and torch.equal(only.data[:, :R], q_t.data[:, :R])
+
+
+def test_cast_of_strided_and_unaligned_inputs():
+    x = _rand(70, 300)
+    for view in (x[:, 4:260], x[3:, :256], x[::2, 8:136], x[:, 1:257], x.t()[:, :64], x[:8].t()[:64].float()):
+        q, q_t = fb.quantize_fp8_block(view, want_t=True)
+        e, e_t = fb.quantize_fp8_block(view.cpu(), want_t=True)
+        _same_bytes(q, e)
+        _same_bytes(q_t, e_t)
+
+
+SHAPES = [(1, 128, 128), (1, 8, 16), (5, 264, 272), (16, 128, 1024), (17, 136, 520), (33, 1000, 640), (64, 256, 4096),
+          (65, 512, 2560), (128, 128, 128), (129, 257, 144), (300, 264, 208), (500, 384, 1920), (1, 2560, 9728),
+          (12, 4096, 2560), (1000, 1032, 1040)]
+
+
+@pytest.mark.parametrize("M,N,K", SHAPES)
+@pytest.mark.parametrize("tile", [False, True])
+def test_product(M, N, K, tile):
+    a, _ = fb.quantize_fp8_block(_rand(M, K))
+    b, _ = fb.quantize_fp8_block(_rand(N, K, seed=1), tile=tile)
+    for dt in (torch.bfloat16, torch.float32):
+        c = fb.matmul_fp8_block(a, b, out_dtype=dt)
+        nv.check_status()
+        assert c.dtype == dt and c.shape == (M, N)
+        _check_product(c, a, b)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 264, 272), (200, 384, 1040)])
+@pytest.mark.parametrize("formats", [(True, False), (False, True), (True, True)])
+def test_product_of_either_format(M, N, K, formats):
+    a, _ = fb.quantize_fp8_block(_rand(M, K), e5m2=formats[0])
+    b, _ = fb.quantize_fp8_block(_rand(N, K, seed=1), e5m2=formats[1])
+    _check_product(fb.matmul_fp8_block(a, b, out_dtype=torch.float32), a, b)
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 136, 640), (150, 256, 272), (700, 520, 1040)])
+def test_bias_accumulation_and_outputs_within_a_larger_tensor(M, N, K):
+    a, _ = fb.quantize_fp8_block(_rand(M, K))
+    b, _ = fb.quantize_fp8_block(_rand(N, K, seed=1), tile=True)
+    bias = _rand(N, spread=0.5)
+    _check_product(fb.matmul_fp8_block(a, b, bias=bias), a, b, bias)
+    _check_product(fb.matmul_fp8_block(a, b, bias=bias, out_dtype=torch.float32), a, b, bias)
+    for dt in (torch.bfloat16, torch.float32):
+        wide = torch.full((M + 2, N + 24), 7.0, dtype=dt, device="cuda")
+        out = wide[1:M + 1, 8:N + 8]
+        assert fb.matmul_fp8_block(a, b, out=out) is out
+        _check_product(out, a, b)
+        kept = wide.clone()
+        kept[1:M + 1, 8:N + 8] = 7
+        assert (kept == 7).all()                 # nothing around it
+    base = torch.randn(M, N, device="cuda")
+    out = base.clone()
+    fb.matmul_fp8_block(a, b, out=out, accumulate=True)
+    _check_product(out, a, b, base=base)
+
+
+def test_parts_of_a_cast_matrix():
+    """Rows of a kept weight (the gate half of a fused one) are a weight of their own."""
+    a, _ = fb.quantize_fp8_block(_rand(40, 640))
+    b, _ = fb.quantize_fp8_block(_rand(384, 640, seed=1), tile=True)
+    for lo, hi in ((0, 128), (128, 384), (200, 201)):
+        part = fb.Fp8BlockTensor(b.data[lo:hi], 640, b.scales[:, lo:hi])
+        _check_product(fb.matmul_fp8_block(a, part), a, part)
+
+
+def test_values_that_are_not_finite_stay_in_their_rows():
+    x = _rand(6, 384)
+    x[2, 130], x[4, 0] = float("nan"), float("inf")
+    a, _ = fb.quantize_fp8_block(x)
+    b, _ = fb.quantize_fp8_block(_rand(128, 384, seed=1), tile=True)
+    c = fb.matmul_fp8_block(a, b)
+    assert torch.isnan(c[[2, 4]]).all() and torch.isfinite(c[[0, 1, 3, 5]]).all()
+
+
+def test_scales_over_their_whole_range():
+    """Factors from 2^-100 to 2^100 on either side: the product of two scales is what counts."""
+    for ea, eb in ((-100, 90), (100, -110), (-60, -50), (50, 40)):
+        a, _ = fb.quantize_fp8_block((_rand(9, 256, spread=0.5).float() * 2.0 ** ea).to(torch.bfloat16))
+        b, _ = fb.quantize_fp8_block((_rand(136, 256, seed=1, spread=0.5).float() * 2.0 ** eb).to(torch.bfloat16))
+        _check_product(fb.matmul_fp8_block(a, b, out_dtype=torch.float32), a, b)
+
+
+def test_refusals_and_empty_products():
+    with pytest.raises(ValueError, match="multiple of 8"):
+        fb.quantize_fp8_block(torch.zeros(4, 12, device="cuda"))
+    q, _ = fb.quantize_fp8_block(torch.zeros(4, 64, device="cuda"))
+    with pytest.raises(ValueError, match="on cuda"):
+        fb.matmul_fp8_block(q, q, out=torch.zeros(4, 4))
+    with pytest.raises(ValueError, match="16 bytes"):
+        fb.matmul_fp8_block(q, fb.Fp8BlockTensor(torch.zeros(4, 72, dtype=torch.uint8, device="cuda")[:, :64], 64, q.scales))
+    e, e_t = fb.quantize_fp8_block(torch.empty(0, 64, device="cuda"), want_t=True)
+    assert fb.matmul_fp8_block(e, q).shape == (0, 4)
+    assert not fb.matmul_fp8_block(e_t, e_t).any()
+    bias = torch.arange(64, device="cuda").to(torch.bfloat16)
+    assert torch.equal(fb.matmul_fp8_block(e_t, e_t, bias=bias), bias.expand(64, 64))
+
+
+# ------------------------------------------------------------------------------------------------
+# Layers
+# ------------------------------------------------------------------------------------------------
+def _value(v, rows, cols):
+    """What a matrix stands for once it is cast (the cast has tests of its own), in 64 bits."""
+    v = v.detach()
+    if rows == 1:
+        return fb.quantize_fp8_block(v)[0].dequantize().double()
+    if cols == 1:
+        return fb.quantize_fp8_block(v, want=False, want_t=True)[1].dequantize().t().double()
+    return fb.quantize_fp8_block(v, tile=True)[0].dequantize().double()
+
+
+def _off(a, b):
+    return float((a.double() - b).norm() / b.norm().clamp(min=1e-300))
+
+
+TOKENS = [1, 2, 15, 64, 129, 333, 1000]
+
+
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("K,N,bias", [(136, 264, True), (1024, 512, False), (640, 72, True)])
+def test_linear_forward_and_gradients(T, K, N, bias):
+    x, w, dy = _rand(T, K, spread=1.0), _rand(N, K, seed=1, spread=0.5), _rand(T, N, seed=2, spread=1.0)
+    b = _rand(N, seed=3, spread=0.5) if bias else None
+    leaves = [t.requires_grad_() for t in (x, w, b) if t is not None]
+    y = fb.linear_fp8_block(x, w, b)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    nv.check_status()
+    wv = _value(w, 128, 128)
+    want = [_value(x, 1, 128) @ wv.t() + (0 if b is None else b.detach().double()), _value(dy, 1, 128) @ wv,
+            _value(dy, 128, 1).t() @ _value(x, 128, 1)] + ([] if b is None else [dy.double().sum(0)])
+    for a, c in zip(got, want):      # bf16 outputs: half a step, 2^-8 of a value, at most
+        assert a.dtype == torch.bfloat16 and a.shape == c.shape and _off(a, c) < 2.0 ** -8
+    with torch.no_grad():
+        q, _ = fb.quantize_fp8_block(w, tile=True)
+        assert torch.equal(fb.linear_fp8_block(x, q, b), y)
+
+
+def test_linear_of_other_types_and_shapes():
+    x, w = _rand(2, 3, 5, 128, spread=0.5).float(), _rand(64, 128, spread=0.5).float()
+    y = fb.linear_fp8_block(x.requires_grad_(), w.requires_grad_())
+    assert y.dtype == torch.float32 and y.shape == (2, 3, 5, 64)
+    y.sum().backward()
+    assert x.grad.dtype == w.grad.dtype == torch.float32 and x.grad.shape == x.shape
+    e = fb.linear_fp8_block(torch.empty(0, 128, device="cuda", dtype=torch.bfloat16), w)
+    assert e.shape == (0, 64)
+
+
+def test_weight_gradients_go_to_the_accumulator():
+    x, w, dy = _rand(300, 256, spread=1.0), _rand(384, 256, seed=1, spread=0.5), _rand(300, 384, seed=2, spread=1.0)
+    w.requires_grad_()
+    w.main_grad = torch.full((384, 256), 3.0, device="cuda")
+    fb.linear_fp8_block(x, w).backward(dy)
+    want = _value(dy, 128, 1).t() @ _value(x, 128, 1)
+    assert w.grad is None and _off(w.main_grad - 3, want) < 1e-5
+
+
+@pytest.mark.parametrize("kind", ["swiglu", "geglu"])
+@pytest.mark.parametrize("T,I", [(1, 128), (100, 384), (128, 256), (259, 640)])
+def test_cast_activations_have_the_bytes_of_the_separate_steps(T, I, kind):
+    from lset_b200.ops.activation import glu
+
+    gu, dh = _rand(T, 2 * I, spread=1.0).requires_grad_(), _rand(T, I, seed=1, spread=1.0)
+    h = glu(gu, kind)
+    (dgu,) = torch.autograd.grad(h, gu, dh)
+    gu, h = gu.detach(), h.detach()
+    with torch.no_grad():
+        _same_bytes(fb._glu_forward(gu, kind), _cpu(fb.quantize_fp8_block(h)[0]))
+        d, d_t, h_t = fb._glu_backward(dh, gu, kind, True, True, True)
+        want, want_t = fb.quantize_fp8_block(dgu, want_t=True)
+        _same_bytes(d, _cpu(want))
+        _same_bytes(d_t, _cpu(want_t))
+        _same_bytes(h_t, _cpu(fb.quantize_fp8_block(h, want=False, want_t=True)[1]))
+
+
+def _cpu(q):
+    return fb.Fp8BlockTensor(q.data.cpu(), q.cols, q.scales.cpu(), q.e5m2)
+
+
+def _mlp_want(x, wgu, wd, kind, dy):
+    bf = lambda v: v.to(torch.bfloat16)  # noqa: E731
+    I = wd.shape[1]
+    wv, dv = _value(wgu, 128, 128), _value(wd, 128, 128)
+    gu = bf(_value(x, 1, 128) @ wv.t()).double().requires_grad_()
+    act = torch.nn.functional.silu if kind == "swiglu" else lambda g: torch.nn.functional.gelu(g, approximate="tanh")
+    h = act(gu[:, :I]) * gu[:, I:]
+    hb, dh = bf(h.detach()), bf(_value(dy, 1, 128) @ dv).double()
+    dgu = bf(torch.autograd.grad(h, gu, dh)[0])
+    return [_value(hb, 1, 128) @ dv.t(), _value(dgu, 1, 128) @ wv, _value(dgu, 128, 1).t() @ _value(x, 128, 1),
+            _value(dy, 128, 1).t() @ _value(hb, 128, 1)]
+
+
+@pytest.mark.parametrize("T", TOKENS)
+@pytest.mark.parametrize("H,I,kind", [(72, 128, "swiglu"), (264, 384, "geglu"), (1024, 1152, "swiglu")])
+def test_gated_mlp_forward_and_gradients(T, H, I, kind):
+    x, dy = _rand(T, H, spread=0.5), _rand(T, H, seed=1, spread=1.0)
+    w, wd = _rand(2 * I, H, seed=2, spread=0.3), _rand(H, I, seed=3, spread=0.3)
+    w, wd = (w.float() * H ** -0.5).to(torch.bfloat16), (wd.float() * I ** -0.5).to(torch.bfloat16)
+    want = _mlp_want(x, w, wd, kind, dy)
+    leaves = [t.requires_grad_() for t in (x, w, wd)]
+    y = fb.gated_mlp_fp8_block(x, w, None, wd, kind)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    nv.check_status()
+    # 2^-8 of a value for the bf16 output, and as much of a norm for values in between that fall to the other side
+    # of a rounding when sums are taken in another order
+    for a, c in zip(got, want):
+        assert a.dtype == torch.bfloat16 and a.shape == c.shape and _off(a, c) < 2.0 ** -7
+    with torch.no_grad():
+        kept = [fb.quantize_fp8_block(t, tile=True)[0] for t in (w, wd)]
+        assert torch.equal(fb.gated_mlp_fp8_block(x, kept[0], None, kept[1], kind), y)
+    halves = [t.detach().clone().requires_grad_() for t in (w[:I], w[I:])]
+    y2 = fb.gated_mlp_fp8_block(x, *halves, wd, kind)
+    g2 = torch.autograd.grad(y2, [x, *halves, wd], dy)
+    assert torch.equal(y2, y) and torch.equal(g2[0], got[1]) and torch.equal(g2[3], got[3])
+    # (a product of half the rows may add its sums in another order: the same bound against the formula, then)
+    assert _off(torch.cat([g2[1], g2[2]]), want[2]) < 2.0 ** -7
