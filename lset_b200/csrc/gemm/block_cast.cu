@@ -10,6 +10,7 @@
 
 #include "../common/pdl.h"
 #include "../row/glu.cuh"
+#include "block_gemm.h"
 #include "block_scale.cuh"
 
 namespace lb {
@@ -19,14 +20,6 @@ using bf16 = __nv_bfloat16;
 
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-
-template <int E5M2>
-__device__ __forceinline__ uint32_t cvt4(float a, float b, float c, float d) {
-  constexpr __nv_fp8_interpretation_t kind = E5M2 ? __NV_E5M2 : __NV_E4M3;
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, kind);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, kind);
-  return lo | (hi << 16);
-}
 
 // The bytes of four words of a 4 x 4 block, transposed.
 __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
@@ -143,8 +136,8 @@ __device__ __forceinline__ void cast_tile(const uint4 (&v)[2][4], CastSmem& sm, 
         if (r < R) {
           if (c < C) {
             const uint4& q = v[u][i];
-            uint2 b = make_uint2(cvt4<E5M2>(bf16_lo(q.x) * s, bf16_hi(q.x) * s, bf16_lo(q.y) * s, bf16_hi(q.y) * s),
-                                 cvt4<E5M2>(bf16_lo(q.z) * s, bf16_hi(q.z) * s, bf16_lo(q.w) * s, bf16_hi(q.w) * s));
+            uint2 b = make_uint2(cast4<E5M2>(bf16_lo(q.x) * s, bf16_hi(q.x) * s, bf16_lo(q.y) * s, bf16_hi(q.y) * s),
+                                 cast4<E5M2>(bf16_lo(q.z) * s, bf16_hi(q.z) * s, bf16_lo(q.w) * s, bf16_hi(q.w) * s));
             if (!ok) b = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
             *reinterpret_cast<uint2*>(out.data + (long long)r * out.ld + c) = b;
           }
@@ -179,7 +172,7 @@ __device__ __forceinline__ void cast_tile(const uint4 (&v)[2][4], CastSmem& sm, 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t a = k ? v[u][i].z : v[u][i].x, b = k ? v[u][i].w : v[u][i].y;
-        q[i] = cvt4<E5M2>(bf16_lo(a) * cs[4 * k], bf16_hi(a) * cs[4 * k + 1], bf16_lo(b) * cs[4 * k + 2],
+        q[i] = cast4<E5M2>(bf16_lo(a) * cs[4 * k], bf16_hi(a) * cs[4 * k + 1], bf16_lo(b) * cs[4 * k + 2],
                           bf16_hi(b) * cs[4 * k + 3]);
       }
       transpose4(q);
@@ -212,10 +205,12 @@ __device__ __forceinline__ void load_tile(uint4 (&v)[2][4], const bf16* __restri
     }
 }
 
+// colsum (where it is wanted: the gradient of a bias): the tile's column sums to row r0 / 128 of a matrix
+// [.., C], always added in the same order.
 template <int TILED, int E5M2>
 __global__ void __launch_bounds__(256)
     block_cast_kernel(const bf16* __restrict__ x, int R, int C, long long ldx, BlockOut out, BlockOut out_t,
-                      int tiles_c) {
+                      float* __restrict__ colsum, int tiles_c) {
   __shared__ __align__(16) CastSmem sm;
   pdl_wait();
   pdl_trigger();
@@ -223,6 +218,34 @@ __global__ void __launch_bounds__(256)
   const int r0 = rt * kTile, c0 = (blockIdx.x - rt * tiles_c) * kTile;
   uint4 v[2][4];
   load_tile(v, x, ldx, r0, c0, R, C);
+  if (!TILED && colsum != nullptr) {
+    float s[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      s[j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint4& q = v[k / 4][k % 4];
+        const uint32_t w = j / 2 == 0 ? q.x : (j / 2 == 1 ? q.y : (j / 2 == 2 ? q.z : q.w));
+        s[j] += j & 1 ? bf16_hi(w) : bf16_lo(w);
+      }
+      s[j] += __shfl_xor_sync(0xffffffffu, s[j], 16);
+    }
+    float* part = reinterpret_cast<float*>(sm.tile);   // [8 warps][128 columns]
+    const int warp = threadIdx.x >> 5, cg = threadIdx.x & 15;
+    if ((threadIdx.x & 31) < 16) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) part[warp * kTile + cg * 8 + j] = s[j];
+    }
+    __syncthreads();
+    if (threadIdx.x < kTile && c0 + threadIdx.x < C) {
+      float t = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t += part[k * kTile + threadIdx.x];
+      colsum[(long long)rt * C + c0 + threadIdx.x] = t;
+    }
+    __syncthreads();
+  }
   cast_tile<TILED, E5M2>(v, sm, r0, c0, R, C, out, out_t);
 }
 
@@ -281,11 +304,109 @@ __global__ void __launch_bounds__(256, 2)
   cast_tile<0, 0>(x, sm, r0, c0, T, I, BlockOut{}, h_t);
 }
 
-BlockOut block_out(void* data, long long ld, void* scales, long long rows, int kb0 = 0) {
-  return BlockOut{static_cast<uint8_t*>(data), ld, static_cast<uint32_t*>(scales), rows, kb0};
+// out [rows, cols] = (out +) sums of P matrices, part p at p * stride, each value in the order of p.
+template <typename OutT>
+__global__ void __launch_bounds__(256)
+    block_sum_kernel(const float* __restrict__ part, int P, long long stride, int rows, int cols, OutT* out,
+                     long long ldo, int accumulate) {
+  pdl_wait();
+  pdl_trigger();
+  const int vecs = cols / 4;
+  const long long n = 1LL * rows * vecs;
+  for (long long i = 1LL * blockIdx.x * blockDim.x + threadIdx.x; i < n; i += 1LL * gridDim.x * blockDim.x) {
+    const long long r = i / vecs;
+    const int c = int(i - r * vecs) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int p = 0; p < P; ++p) {
+      const float4 v = *reinterpret_cast<const float4*>(part + p * stride + 4 * i);
+      s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    OutT* o = out + r * ldo + c;
+    if constexpr (sizeof(OutT) == 2) {
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(s.x, s.y), pack_bf16x2(s.z, s.w));
+    } else {
+      float4* o4 = reinterpret_cast<float4*>(o);
+      if (accumulate) {
+        const float4 v = *o4;
+        s = make_float4(v.x + s.x, v.y + s.y, v.z + s.z, v.w + s.w);
+      }
+      *o4 = s;
+    }
+  }
+}
+
+BlockOut block_out(const BlockMat& m, int kb0 = 0) { return BlockOut{m.data, m.ld, m.scales, m.rows_s, kb0}; }
+
+// CTAs of the tiles of [R, C]; 0 where there are too many.
+unsigned cast_grid(int R, int C) {
+  const long long tiles = 1LL * ((C + kTile - 1) / kTile) * ((R + kTile - 1) / kTile);
+  return tiles > 0x7fffffffLL ? 0u : unsigned(tiles);
+}
+
+bool fits(const BlockMat& m, long long rows, long long cols) {
+  return m.data == nullptr || (!(m.ld & 15) && m.ld >= cols && m.rows_s >= rows && m.scales != nullptr);
 }
 
 }  // namespace
+
+int block_cast(const void* x, int R, int C, long long ldx, int tiled, int e5m2, const BlockMat& out,
+               const BlockMat& out_t, int kb0_t, float* colsum, cudaStream_t stream) {
+  if (R <= 0 || C <= 0) return 0;
+  if ((C & 7) || (ldx & 7) || (reinterpret_cast<uintptr_t>(x) & 15)) return -3;
+  if (!fits(out, R, C) || !fits(out_t, C, R) || kb0_t < 0 || (kb0_t > 0 && (R % kTile))) return -3;
+  if (colsum != nullptr && tiled) return -5;
+  const unsigned grid = cast_grid(R, C);
+  if (grid == 0) return -3;
+  auto kern = tiled ? (e5m2 ? block_cast_kernel<1, 1> : block_cast_kernel<1, 0>)
+                    : (e5m2 ? block_cast_kernel<0, 1> : block_cast_kernel<0, 0>);
+  return launch_pdl(kern, dim3(grid), dim3(256), 0, stream, pdl_enabled(4LL * R * C), 1,
+                    static_cast<const bf16*>(x), R, C, ldx, block_out(out), block_out(out_t, kb0_t), colsum,
+                    (C + kTile - 1) / kTile);
+}
+
+// h = act(gate) * up of [T, I] (rows ld elements apart; I a multiple of 128) in blocks of a row. kind: 0 = SwiGLU,
+// 1 = GeGLU (tanh).
+int block_glu_fwd(int kind, const void* gate, const void* up, long long ld, int T, int I, const BlockMat& out,
+                  cudaStream_t stream) {
+  if (T <= 0 || I <= 0) return 0;
+  if ((I % kTile) || (ld & 7) || !fits(out, T, I)) return -3;
+  const unsigned grid = cast_grid(T, I);
+  if (grid == 0) return -3;
+  return launch_pdl(kind == kSwiglu ? block_glu_fwd_kernel<kSwiglu> : block_glu_fwd_kernel<kGeglu>, dim3(grid),
+                    dim3(256), 0, stream, pdl_enabled(5LL * T * I), 1, static_cast<const bf16*>(gate),
+                    static_cast<const bf16*>(up), ld, T, I, block_out(out), I / kTile);
+}
+
+// From dh [T, I], gate and up: `d` [T, 2 I] and `d_t` [2 I, T], the gradients of gate and up, and `h_t` [I, T].
+int block_glu_bwd(int kind, const void* dh, long long ld_dh, const void* gate, const void* up, long long ld,
+                  int T, int I, const BlockMat& d, const BlockMat& d_t, const BlockMat& h_t,
+                  cudaStream_t stream) {
+  if (T <= 0 || I <= 0) return 0;
+  if ((I % kTile) || (ld & 7) || (ld_dh & 7)) return -3;
+  if (!fits(d, T, 2LL * I) || !fits(d_t, 2LL * I, T) || !fits(h_t, I, T)) return -3;
+  const unsigned grid = cast_grid(T, I);
+  if (grid == 0) return -3;
+  return launch_pdl(kind == kSwiglu ? block_glu_bwd_kernel<kSwiglu> : block_glu_bwd_kernel<kGeglu>, dim3(grid),
+                    dim3(256), 0, stream, pdl_enabled(11LL * T * I), 1, static_cast<const bf16*>(dh), ld_dh,
+                    static_cast<const bf16*>(gate), static_cast<const bf16*>(up), ld, T, I, block_out(d),
+                    block_out(d_t), block_out(h_t), I / kTile);
+}
+
+// cols a multiple of 4; part, stride and out 16-byte aligned (out: 8 bytes in bf16).
+int block_sum(const float* part, int P, long long stride, int rows, int cols, void* out, long long ldo,
+              int out_fp32, int accumulate, cudaStream_t stream) {
+  if (rows <= 0 || cols <= 0) return 0;
+  if ((cols & 3) || (stride & 3) || (ldo & 3) || (accumulate && !out_fp32)) return -3;
+  const long long n = 1LL * rows * (cols / 4);
+  const unsigned grid = unsigned(n > 148LL * 8 * 256 ? 148 * 8 : (n + 255) / 256);
+  const bool pdl = pdl_enabled(4LL * P * rows * cols);
+  return out_fp32 ? launch_pdl(block_sum_kernel<float>, dim3(grid), dim3(256), 0, stream, pdl, 1, part, P, stride,
+                               rows, cols, static_cast<float*>(out), ldo, accumulate)
+                  : launch_pdl(block_sum_kernel<bf16>, dim3(grid), dim3(256), 0, stream, pdl, 1, part, P, stride,
+                               rows, cols, static_cast<bf16*>(out), ldo, 0);
+}
+
 }  // namespace lb
 
 // x [R, C] (bf16, rows ldx elements apart; C and ldx multiples of 8, x 16-byte aligned) in 8 bits: `out` [R, C]
@@ -297,59 +418,8 @@ BlockOut block_out(void* data, long long ld, void* scales, long long rows, int k
 extern "C" int lb_block_cast(const void* x, int R, int C, long long ldx, int tiled, int e5m2, void* out,
                              long long ldo, void* scales, long long rows_s, void* out_t, long long ldt,
                              void* scales_t, long long rows_st, int kb0_t, void* stream_) {
-  using namespace lb;
-  if (R <= 0 || C <= 0) return 0;
-  if ((C & 7) || (ldx & 7) || (reinterpret_cast<uintptr_t>(x) & 15)) return -3;
-  if (out != nullptr && ((ldo & 15) || ldo < C || rows_s < R || scales == nullptr)) return -3;
-  if (out_t != nullptr && ((ldt & 15) || ldt < R || rows_st < C || scales_t == nullptr)) return -3;
-  if (kb0_t < 0 || (kb0_t > 0 && (R % kTile))) return -3;
-  if (out == nullptr && out_t == nullptr) return 0;
-  const int tiles_c = (C + kTile - 1) / kTile;
-  const long long tiles = 1LL * tiles_c * ((R + kTile - 1) / kTile);
-  if (tiles > 0x7fffffffLL) return -3;
-  const BlockOut o = block_out(out, ldo, scales, rows_s);
-  const BlockOut t = block_out(out_t, ldt, scales_t, rows_st, kb0_t);
-  auto kern = tiled ? (e5m2 ? block_cast_kernel<1, 1> : block_cast_kernel<1, 0>)
-                    : (e5m2 ? block_cast_kernel<0, 1> : block_cast_kernel<0, 0>);
-  return launch_pdl(kern, dim3(unsigned(tiles)), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream_),
-                    pdl_enabled(4LL * R * C), 1, reinterpret_cast<const bf16*>(x), R, C, ldx, o, t, tiles_c);
-}
-
-// h = act(gate) * up of [T, I] (rows ld elements apart; I a multiple of 128) in blocks of a row: `out` [T, I]
-// bytes, rows ldo apart; scales [ceil(I / 512)][rows_s]. kind: 0 = SwiGLU, 1 = GeGLU (tanh).
-extern "C" int lb_block_glu_fwd(int kind, const void* gate, const void* up, long long ld, int T, int I, void* out,
-                                long long ldo, void* scales, long long rows_s, void* stream_) {
-  using namespace lb;
-  if (T <= 0 || I <= 0) return 0;
-  if ((I % kTile) || (ld & 7) || (ldo & 15) || ldo < I || rows_s < T) return -3;
-  const int tiles_c = I / kTile;
-  const long long tiles = 1LL * tiles_c * ((T + kTile - 1) / kTile);
-  if (tiles > 0x7fffffffLL) return -3;
-  return launch_pdl(kind == kSwiglu ? block_glu_fwd_kernel<kSwiglu> : block_glu_fwd_kernel<kGeglu>,
-                    dim3(unsigned(tiles)), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream_),
-                    pdl_enabled(5LL * T * I), 1, static_cast<const bf16*>(gate), static_cast<const bf16*>(up), ld, T,
-                    I, block_out(out, ldo, scales, rows_s), tiles_c);
-}
-
-// From dh [T, I], gate and up: `d` [T, 2 I] and `d_t` [2 I, T], the gradients of gate and up, and `h_t` [I, T]
-// (bytes and scale words as lb_block_cast writes them; any may be null).
-extern "C" int lb_block_glu_bwd(int kind, const void* dh, long long ld_dh, const void* gate, const void* up,
-                                long long ld, int T, int I, void* d, long long ldd, void* scales_d,
-                                long long rows_d, void* d_t, long long lddt, void* scales_dt, long long rows_dt,
-                                void* h_t, long long ldht, void* scales_ht, long long rows_ht, void* stream_) {
-  using namespace lb;
-  if (T <= 0 || I <= 0) return 0;
-  if ((I % kTile) || (ld & 7) || (ld_dh & 7)) return -3;
-  if (d != nullptr && ((ldd & 15) || ldd < 2LL * I || rows_d < T)) return -3;
-  if (d_t != nullptr && ((lddt & 15) || lddt < T || rows_dt < 2LL * I)) return -3;
-  if (h_t != nullptr && ((ldht & 15) || ldht < T || rows_ht < I)) return -3;
-  const int tiles_c = I / kTile;
-  const long long tiles = 1LL * tiles_c * ((T + kTile - 1) / kTile);
-  if (tiles > 0x7fffffffLL) return -3;
-  return launch_pdl(kind == kSwiglu ? block_glu_bwd_kernel<kSwiglu> : block_glu_bwd_kernel<kGeglu>,
-                    dim3(unsigned(tiles)), dim3(256), 0, reinterpret_cast<cudaStream_t>(stream_),
-                    pdl_enabled(11LL * T * I), 1, static_cast<const bf16*>(dh), ld_dh,
-                    static_cast<const bf16*>(gate), static_cast<const bf16*>(up), ld, T, I,
-                    block_out(d, ldd, scales_d, rows_d), block_out(d_t, lddt, scales_dt, rows_dt),
-                    block_out(h_t, ldht, scales_ht, rows_ht), tiles_c);
+  return lb::block_cast(x, R, C, ldx, tiled, e5m2,
+                        lb::BlockMat{static_cast<uint8_t*>(out), ldo, static_cast<uint32_t*>(scales), rows_s, e5m2},
+                        lb::BlockMat{static_cast<uint8_t*>(out_t), ldt, static_cast<uint32_t*>(scales_t), rows_st, e5m2},
+                        kb0_t, nullptr, reinterpret_cast<cudaStream_t>(stream_));
 }

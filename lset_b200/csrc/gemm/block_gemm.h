@@ -1,0 +1,62 @@
+// Block-scaled 8-bit products for callers within the library (gemm_block.cu, gemm_block_2cta.cu,
+// block_cast.cu, block_layers.cu).
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+namespace lb {
+
+// An 8-bit matrix [rows, cols]: bytes, rows ld apart, and scale words, `rows_s` of them a group of four
+// blocks (block_scale.cuh).
+struct BlockMat {
+  uint8_t* data;
+  long long ld;
+  uint32_t* scales;
+  long long rows_s;
+  int e5m2;
+};
+
+// How a product runs: kernel 0 is the one-CTA kernel with tiles of 128 x tn and the contraction split over
+// clusters of `splits`; kernel 1 the pair kernel, its contraction split into `splits` fp32 products that a
+// second launch adds up.
+struct BlockPlan {
+  int kernel, tn, splits;
+};
+BlockPlan block_plan(int M, int N, int K, int out_fp32, int accumulate, bool bias, bool aligned);
+// Bytes of temporary storage of a plan.
+size_t block_plan_bytes(const BlockPlan& p, int M, int N);
+
+// C [M, N] = or += A · Bᵀ + bias; ws: block_plan_bytes.
+int block_gemm(const BlockPlan& p, const BlockMat& A, const BlockMat& B, void* C, int M, int N, int K,
+               long long ldc, int out_fp32, int accumulate, const void* bias, void* ws, int* status,
+               cudaStream_t stream);
+
+int block_gemm_1cta(int tn, int splits, const BlockMat& A, const BlockMat& B, void* C, int M, int N, int K,
+                    long long ldc, int out_fp32, int accumulate, const void* bias, int* status,
+                    cudaStream_t stream);
+int block_gemm_2cta(int splits, long long split_stride, const BlockMat& A, const BlockMat& B, void* C, int M,
+                    int N, int K, long long ldc, int out_fp32, int accumulate, const void* bias, int* status,
+                    cudaStream_t stream);
+// Whether `splits` divides the contraction into that many parts (whole groups of scale words each).
+bool block_2cta_splits_ok(int K, int splits);
+int block_2cta_pairs();
+// h = act(A · Wgᵀ) * (A · Wuᵀ), cast; Wu's rows follow Wg's scale words in one group. See gemm_block_2cta.cu.
+int block_gemm_glu(int kind, const BlockMat& A, const BlockMat& Wg, const BlockMat& Wu, int M, int I, int K,
+                   void* gate, void* up, long long ld_gu, const BlockMat& h, int* status, cudaStream_t stream);
+
+// block_cast.cu. Casts of x [R, C] as rows and / or transposed (data null: not wanted). colsum: fp32
+// [ceil(R / 128)][C], the column sums of each 128 rows of x (null: not wanted).
+int block_cast(const void* x, int R, int C, long long ldx, int tiled, int e5m2, const BlockMat& out,
+               const BlockMat& out_t, int kb0_t, float* colsum, cudaStream_t stream);
+int block_glu_fwd(int kind, const void* gate, const void* up, long long ld, int T, int I, const BlockMat& out,
+                  cudaStream_t stream);
+int block_glu_bwd(int kind, const void* dh, long long ld_dh, const void* gate, const void* up, long long ld,
+                  int T, int I, const BlockMat& d, const BlockMat& d_t, const BlockMat& h_t,
+                  cudaStream_t stream);
+// out [rows, cols] (bf16 or fp32, rows ldo apart) = or += the sum of P matrices [rows, cols] of fp32, in order.
+int block_sum(const float* part, int P, long long stride, int rows, int cols, void* out, long long ldo,
+              int out_fp32, int accumulate, cudaStream_t stream);
+
+}  // namespace lb

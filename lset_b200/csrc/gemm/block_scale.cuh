@@ -39,6 +39,15 @@ __device__ __forceinline__ bool block_is_finite(uint32_t a) { return a < 0x7f80u
 // 2^(127 - e): what a value is multiplied by before it is rounded.
 __device__ __forceinline__ float block_inverse(uint32_t e) { return __uint_as_float((254u - e) << 23); }
 
+// Four values, scaled already, as bytes.
+template <int E5M2>
+__device__ __forceinline__ uint32_t cast4(float a, float b, float c, float d) {
+  constexpr __nv_fp8_interpretation_t kind = E5M2 ? __NV_E5M2 : __NV_E4M3;
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, kind);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, kind);
+  return lo | (hi << 16);
+}
+
 // D[tmem] (+)= (A[smem] * scales) * (B[smem] * scales), 8-bit floats, 32 elements of depth. The scale
 // operands are tensor-memory addresses: row r's word lies in lane r % 32 (of every quarter of the lanes),
 // column r / 32; the instruction descriptor says which of its bytes applies.

@@ -31,6 +31,7 @@
 #include <cuda_bf16.h>
 #include <stdlib.h>
 
+#include "../common/pair.cuh"
 #include "../common/pdl.h"
 #include "../common/ptx.cuh"
 #include "../common/tma_desc.h"
@@ -94,54 +95,6 @@ struct Args2 {
   int* status;
 };
 
-__device__ __forceinline__ uint32_t cluster_ctarank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_sync_all() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// Address of `p` (own shared memory) as seen in CTA `rank` of the cluster.
-__device__ __forceinline__ uint32_t map_to_cta(const void* p, uint32_t rank) {
-  uint32_t out;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(out) : "r"(smem_u32(p)), "r"(rank));
-  return out;
-}
-// Arrival on a barrier of the partner CTA. No data written by this thread is handed over with it
-// (the barriers of this kernel order TMA writes, tensor-core reads and TMEM reads, all of which
-// complete before the arrival is issued), so the default semantics are enough; cluster-scope
-// acquire / release on the per-stage path costs a fence per k-block in the issuing threads.
-__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-// 2-D tile load into this CTA's shared memory whose completion bytes are counted on `bar_cluster`,
-// a barrier of either CTA of the pair (cluster address).
-__device__ __forceinline__ void tma_load_2d_pair(void* smem_dst, const CUtensorMap* tm,
-                                                 uint32_t bar_cluster, int x, int y) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes "
-      "[%0], [%1, {%3, %4}], [%2];"
-      :
-      : "r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar_cluster), "r"(x),
-        "r"(y)
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_alloc2(uint32_t* smem_slot, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   smem_u32(smem_slot)),
-               "r"(ncols)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish2() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
-               : "memory");
-}
 // D (both CTAs' tensor memory) (+)= A (both CTAs' smem) * B (both CTAs' smem); leader thread only.
 __device__ __forceinline__ void umma2_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc,
                                            uint32_t idesc, uint32_t accumulate) {
@@ -167,27 +120,9 @@ __device__ __forceinline__ void umma2_f8(uint32_t tmem_d, uint64_t adesc, uint64
       : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// Arrive on the barrier at this shared-memory offset in both CTAs of the pair once the tcgen05
-// operations issued so far have completed: one commit per CTA, the peer's barrier through its
-// address in the cluster's shared-memory window.
-__device__ __forceinline__ void umma2_commit_both(uint64_t* bar, uint32_t peer_rank) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   smem_u32(bar))
-               : "memory");
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-                   map_to_cta(bar, peer_rank))
-               : "memory");
-}
-
 __device__ __forceinline__ void red_add8_bf16(void* dst, const uint4& v) {
   asm volatile("red.global.add.noftz.v4.bf16x2 [%0], {%1, %2, %3, %4};" ::"l"(dst), "r"(v.x),
                "r"(v.y), "r"(v.z), "r"(v.w)
-               : "memory");
-}
-
-__device__ __forceinline__ void red_add4(float* dst, float a, float b, float c, float d) {
-  asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(dst), "f"(a), "f"(b), "f"(c),
-               "f"(d)
                : "memory");
 }
 

@@ -16,6 +16,7 @@
 #include "../common/pdl.h"
 #include "../common/ptx.cuh"
 #include "../common/tma_desc.h"
+#include "block_gemm.h"
 #include "block_scale.cuh"
 
 namespace lb {
@@ -281,54 +282,105 @@ int launch_block(const CUtensorMap& tmP, const CUtensorMap& tmQ, const BlockArgs
 }
 
 }  // namespace
-}  // namespace lb
 
-// C [M, N] (bf16 or fp32, rows ldc elements apart) = A · Bᵀ + bias for A [M, K] and B [N, K] in 8 bits
-// (bytes, rows lda / ldb apart, multiples of 16; e5m2 or e4m3) with scale words sa [ceil(K / 512)][rows_sa]
-// and sb [..][rows_sb]. accumulate (fp32 only, no bias): C += A · Bᵀ.
-extern "C" int lb_gemm_block(const void* A, const void* B, void* C, int M, int N, int K, long long lda,
-                             long long ldb, long long ldc, int a_e5m2, int b_e5m2, const void* sa,
-                             long long rows_sa, const void* sb, long long rows_sb, int out_fp32, int accumulate,
-                             const void* bias, int* status, void* stream_) {
-  using namespace lb;
-  if (M <= 0 || N <= 0) return 0;
-  if (K <= 0) return -4;
-  if ((lda & 15) || (ldb & 15) || lda < K || ldb < K || ldc < N || rows_sa < M || rows_sb < N) return -3;
-  if (accumulate && (!out_fp32 || bias != nullptr)) return -5;
-  const int tn = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
+int block_gemm_1cta(int tn, int splits, const BlockMat& A, const BlockMat& B, void* C, int M, int N, int K,
+                    long long ldc, int out_fp32, int accumulate, const void* bias, int* status,
+                    cudaStream_t stream) {
+  const int kb = (K + kScaleBlock - 1) / kScaleBlock;
+  if (splits < 1 || splits > 8 || splits > kb) return -5;
   BlockArgs g{};
   g.M = M;
   g.N = N;
   g.K = K;
-  g.sa = static_cast<const uint32_t*>(sa);
-  g.sb = static_cast<const uint32_t*>(sb);
-  g.rows_sa = rows_sa;
-  g.rows_sb = rows_sb;
+  g.sa = A.scales;
+  g.sb = B.scales;
+  g.rows_sa = A.rows_s;
+  g.rows_sb = B.rows_s;
   g.C = C;
   g.ldc = ldc;
   g.out_fp32 = out_fp32;
   g.accumulate = accumulate;
   g.bias = static_cast<const __nv_bfloat16*>(bias);
-  g.a_e5m2 = a_e5m2 ? 1 : 0;
-  g.b_e5m2 = b_e5m2 ? 1 : 0;
+  g.a_e5m2 = A.e5m2 ? 1 : 0;
+  g.b_e5m2 = B.e5m2 ? 1 : 0;
   g.q_rows = M < tn ? M : tn;
   g.tiles_m = (M + tn - 1) / tn;
   g.status = status;
   const long long tiles = 1LL * g.tiles_m * ((N + kBP - 1) / kBP);
-  const int kb = (K + kScaleBlock - 1) / kScaleBlock;
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 2 * 148 && kb >= 4 * splits) splits *= 2;
   if (tiles * splits > 0x7fffffffLL) return -3;
   CUtensorMap tmP, tmQ;
-  int rc = make_tmap_2d(&tmP, B, 1, (uint64_t)K, (uint64_t)N, (uint64_t)ldb, 128, kBP, true);
+  int rc = make_tmap_2d(&tmP, B.data, 1, (uint64_t)K, (uint64_t)N, (uint64_t)B.ld, 128, kBP, true);
   if (rc) return rc;
-  rc = make_tmap_2d(&tmQ, A, 1, (uint64_t)K, (uint64_t)M, (uint64_t)lda, 128, uint32_t(g.q_rows), true);
+  rc = make_tmap_2d(&tmQ, A.data, 1, (uint64_t)K, (uint64_t)M, (uint64_t)A.ld, 128, uint32_t(g.q_rows), true);
   if (rc) return rc;
-  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_);
   switch (tn) {
     case 16: return launch_block<16>(tmP, tmQ, g, tiles, splits, stream);
     case 32: return launch_block<32>(tmP, tmQ, g, tiles, splits, stream);
     case 64: return launch_block<64>(tmP, tmQ, g, tiles, splits, stream);
-    default: return launch_block<128>(tmP, tmQ, g, tiles, splits, stream);
+    case 128: return launch_block<128>(tmP, tmQ, g, tiles, splits, stream);
   }
+  return -5;
+}
+
+BlockPlan block_plan(int M, int N, int K, int out_fp32, int accumulate, bool bias, bool aligned) {
+  if (aligned && 1LL * ((M + 255) / 256) * ((N + 255) / 256) >= 40) return BlockPlan{1, 0, 1};
+  const int tn = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
+  const long long tiles = 1LL * ((M + tn - 1) / tn) * ((N + kBP - 1) / kBP);
+  const int kb = (K + kScaleBlock - 1) / kScaleBlock;
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= 2 * 148 && kb >= 4 * splits) splits *= 2;
+  return BlockPlan{0, tn, splits};
+}
+
+size_t block_plan_bytes(const BlockPlan& p, int M, int N) {
+  return p.kernel == 1 && p.splits > 1 ? size_t(p.splits) * M * N * 4 : 0;
+}
+
+int block_gemm(const BlockPlan& p, const BlockMat& A, const BlockMat& B, void* C, int M, int N, int K,
+               long long ldc, int out_fp32, int accumulate, const void* bias, void* ws, int* status,
+               cudaStream_t stream) {
+  if (p.kernel == 0)
+    return block_gemm_1cta(p.tn, p.splits, A, B, C, M, N, K, ldc, out_fp32, accumulate, bias, status, stream);
+  if (p.splits == 1)
+    return block_gemm_2cta(1, 0, A, B, C, M, N, K, ldc, out_fp32, accumulate, bias, status, stream);
+  const long long stride = 1LL * M * N;
+  const int rc = block_gemm_2cta(p.splits, stride, A, B, ws, M, N, K, N, 1, 0, nullptr, status, stream);
+  if (rc) return rc;
+  return block_sum(static_cast<const float*>(ws), p.splits, stride, M, N, C, ldc, out_fp32, accumulate, stream);
+}
+
+}  // namespace lb
+
+namespace {
+bool aligned_for_pairs(const void* C, int N, long long ldc) {
+  return !(N & 7) && !(ldc & 7) && !(reinterpret_cast<uintptr_t>(C) & 15);
+}
+}  // namespace
+
+// Bytes of temporary storage that lb_gemm_block wants for this product (a 16-byte aligned C).
+extern "C" long long lb_gemm_block_bytes(int M, int N, int K, long long ldc, int out_fp32, int accumulate,
+                                         int bias) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return (long long)lb::block_plan_bytes(
+      lb::block_plan(M, N, K, out_fp32, accumulate, bias != 0, aligned_for_pairs(nullptr, N, ldc)), M, N);
+}
+
+// C [M, N] (bf16 or fp32, rows ldc elements apart) = A · Bᵀ + bias for A [M, K] and B [N, K] in 8 bits
+// (bytes, rows lda / ldb apart, multiples of 16; e5m2 or e4m3) with scale words sa [ceil(K / 512)][rows_sa]
+// and sb [..][rows_sb]. accumulate (fp32 only, no bias): C += A · Bᵀ. ws: lb_gemm_block_bytes, 16-byte aligned.
+extern "C" int lb_gemm_block(const void* A, const void* B, void* C, int M, int N, int K, long long lda,
+                             long long ldb, long long ldc, int a_e5m2, int b_e5m2, const void* sa,
+                             long long rows_sa, const void* sb, long long rows_sb, int out_fp32, int accumulate,
+                             const void* bias, void* ws, long long ws_bytes, int* status, void* stream_) {
+  using namespace lb;
+  if (M <= 0 || N <= 0) return 0;
+  if (K <= 0) return -4;
+  if ((lda & 15) || (ldb & 15) || lda < K || ldb < K || ldc < N || rows_sa < M || rows_sb < N) return -3;
+  if (accumulate && (!out_fp32 || bias != nullptr)) return -5;
+  const BlockMat a{(uint8_t*)A, lda, (uint32_t*)sa, rows_sa, a_e5m2};
+  const BlockMat b{(uint8_t*)B, ldb, (uint32_t*)sb, rows_sb, b_e5m2};
+  const BlockPlan p = block_plan(M, N, K, out_fp32, accumulate, bias != nullptr, aligned_for_pairs(C, N, ldc));
+  if (block_plan_bytes(p, M, N) > size_t(ws_bytes)) return -6;
+  return block_gemm(p, a, b, C, M, N, K, ldc, out_fp32, accumulate, bias, ws, status,
+                    reinterpret_cast<cudaStream_t>(stream_));
 }

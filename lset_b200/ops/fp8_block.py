@@ -17,11 +17,14 @@ a row or a column; the recipe ``block128`` of ``train/quantization/fp8.py`` sele
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nv
 from .activation import glu_ref
@@ -89,10 +92,20 @@ def _scale_rows(s: torch.Tensor) -> int:
 _P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 _SIGNATURES = {
     "lb_block_cast": [_P, _I, _I, _L, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _I, _P],
-    "lb_block_glu_fwd": [_I, _P, _P, _L, _I, _I, _P, _L, _P, _L, _P],
-    "lb_block_glu_bwd": [_I, _P, _L, _P, _P, _L, _I, _I] + 3 * [_P, _L, _P, _L] + [_P],
-    "lb_gemm_block": [_P, _P, _P, _I, _I, _I, _L, _L, _L, _I, _I, _P, _L, _P, _L, _I, _I, _P, _P, _P],
+    "lb_gemm_block_bytes": [_I, _I, _I, _L, _I, _I, _I],
+    "lb_gemm_block": [_P, _P, _P, _I, _I, _I, _L, _L, _L, _I, _I, _P, _L, _P, _L, _I, _I, _P, _P, _L, _P, _P],
+    "lb_linear_block_bytes": [_I] * 6 + [_P],
+    "lb_linear_block_fwd": [_P, _L, _P, _L, _P, _I, _I, _I, _I, _I] + [_P] * 5,
+    "lb_linear_block_bwd": [_P, _L, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _P, _I, _P, _P],
+    "lb_linear_kept_bytes": [_I] * 4,
+    "lb_linear_kept_fwd": [_P, _L, _P, _L, _P, _L, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P],
+    "lb_mlp_block_bytes": [_I] * 4 + [_P, _P],
+    "lb_mlp_block_fwd": [_I, _P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I] + [_P] * 5,
+    "lb_mlp_block_bwd": [_I, _P, _L, _I, _I, _I, _I, _I] + [_P] * 9,
+    "lb_mlp_kept_bytes": [_I] * 3,
+    "lb_mlp_kept_fwd": [_I, _P, _L, _P, _L, _P, _L, _I, _P, _L, _P, _L, _I, _I, _I, _I] + [_P] * 4,
 }
+_RETURNS = {"lb_gemm_block_bytes": _L, "lb_linear_kept_bytes": _L, "lb_mlp_kept_bytes": _L}
 _fns = {}
 
 
@@ -101,20 +114,33 @@ def _fn(name):
     f = _fns.get(name)
     if f is None:
         f = getattr(nv.load(), name)
-        f.argtypes, f.restype = _SIGNATURES[name], _I
+        f.argtypes, f.restype = _SIGNATURES[name], _RETURNS.get(name, _I)
         _fns[name] = f
     return f
 
 
+def _call(name, *args):
+    rc = _fn(name)(*args)
+    if rc != 0:
+        nv.check_rc(rc, f"{name}{tuple(a for a in args if a is not None and not a >> 24)}")
+
+
 def _on_device(*tensors):
-    """The tensors' one CUDA device as a context; launches go to the current stream of that device."""
+    """The tensors' one CUDA device as a context: launches go to the current stream of that device."""
     dev = None
     for t in tensors:
         if t is not None:
             if dev is not None and t.device != dev:
                 raise ValueError(f"operands are on {dev} and {t.device}")
             dev = t.device
-    return torch.cuda.device(dev)
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _bytes(n: int, device) -> torch.Tensor:
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -190,15 +216,6 @@ def _where(q: Optional[Fp8BlockTensor]):
     return q.data.data_ptr(), _row_bytes(q.data), q.scales.data_ptr(), _scale_rows(q.scales)
 
 
-def _cast_into(x, tile, e5m2, out: Optional[Fp8BlockTensor], out_t: Optional[Fp8BlockTensor]) -> None:
-    R, C = x.shape
-    rc = _fn("lb_block_cast")(x.data_ptr(), R, C, x.stride(0), tile, e5m2, *_where(out), *_where(out_t), 0,
-                              nv.stream_ptr())
-    if rc != 0:
-        nv.check_rc(rc, f"lb_block_cast(R={R},C={C})")
-    nv.count_launch()
-
-
 def quantize_fp8_block(x: torch.Tensor, *, tile: bool = False, e5m2: bool = False, want: bool = True,
                        want_t: bool = False):
     """Cast a 2-D matrix ``x [R, C]`` (bf16; other types are rounded to it first) to 8 bits in blocks of 128.
@@ -219,25 +236,19 @@ def quantize_fp8_block(x: torch.Tensor, *, tile: bool = False, e5m2: bool = Fals
         x = _aligned(x.detach())
         out = _empty(R, C, e5m2, x.device) if want else None
         out_t = _empty(C, R, e5m2, x.device) if want_t else None
-        if R and C:
-            _cast_into(x, tile, e5m2, out, out_t)
+        if R and C and (want or want_t):
+            _call("lb_block_cast", x.data_ptr(), R, C, x.stride(0), tile, e5m2, *_where(out), *_where(out_t), 0,
+                  nv.stream_ptr())
+            nv.count_launch()
     return out, out_t
 
 
 # ------------------------------------------------------------------------------------------------
 # Products
 # ------------------------------------------------------------------------------------------------
-def _matmul(a: Fp8BlockTensor, b: Fp8BlockTensor, out: torch.Tensor, accumulate: bool, bias) -> None:
-    """The product of checked operands on the current device."""
-    M, N, K = a.data.shape[0], b.data.shape[0], a.cols
-    rc = _fn("lb_gemm_block")(
-        a.data.data_ptr(), b.data.data_ptr(), out.data_ptr(), M, N, K, _row_bytes(a.data), _row_bytes(b.data),
-        out.stride(0) if M > 1 else N, a.e5m2, b.e5m2, a.scales.data_ptr(), _scale_rows(a.scales),
-        b.scales.data_ptr(), _scale_rows(b.scales), out.dtype == torch.float32, accumulate,
-        0 if bias is None else bias.data_ptr(), nv.status_word(out.device).data_ptr(), nv.stream_ptr())
-    if rc != 0:
-        nv.check_rc(rc, f"lb_gemm_block(M={M},N={N},K={K})")
-    nv.count_launch()
+@functools.lru_cache(maxsize=4096)
+def _product_bytes(M, N, K, ldc, fp32, accumulate, bias) -> int:
+    return _fn("lb_gemm_block_bytes")(M, N, K, ldc, fp32, accumulate, bias)
 
 
 def matmul_fp8_block(a: Fp8BlockTensor, b: Fp8BlockTensor, *, out: Optional[torch.Tensor] = None,
@@ -280,56 +291,135 @@ def matmul_fp8_block(a: Fp8BlockTensor, b: Fp8BlockTensor, *, out: Optional[torc
             return out
         if bias is not None:
             bias = bias.to(torch.bfloat16).contiguous()
-        _matmul(a, b, out, accumulate, bias)
+        ldc, fp32 = (out.stride(0) if M > 1 else N), out_dtype == torch.float32
+        n = _product_bytes(M, N, K, ldc, fp32, accumulate, bias is not None)
+        ws = _bytes(n, out.device) if n else None
+        _call("lb_gemm_block", a.data.data_ptr(), b.data.data_ptr(), out.data_ptr(), M, N, K, _row_bytes(a.data),
+              _row_bytes(b.data), ldc, a.e5m2, b.e5m2, a.scales.data_ptr(), _scale_rows(a.scales), b.scales.data_ptr(),
+              _scale_rows(b.scales), fp32, accumulate, nv.ptr(bias), nv.ptr(ws), n,
+              nv.status_word(out.device).data_ptr(), nv.stream_ptr())
+        nv.count_launch()
     return out
 
 
 # ------------------------------------------------------------------------------------------------
 # Layers
 # ------------------------------------------------------------------------------------------------
-def _weight_gradient(w, a_t: Fp8BlockTensor, b_t: Fp8BlockTensor):
-    """``dyᵀ · x`` into the weight's fp32 accumulator (returns None), or in the weight's type."""
+_BF16, _FP32, _ADD = 0, 1, 2     # where a result goes: a bf16 or fp32 tensor, or added to an fp32 one
+
+
+def _mode(dtype) -> int:
+    return _FP32 if dtype == torch.float32 else _BF16
+
+
+def _gradient_of(w):
+    """``(tensor, mode)`` that a native call writes the gradient of weight ``w`` to: its fp32 accumulator where the
+    sharding runtime has given it one, else a tensor of its type (fp32 for types other than bf16)."""
     main = main_grad_of(w)
-    if main is not None and a_t.data.is_cuda:
-        matmul_fp8_block(a_t, b_t, out=main, accumulate=True)
-        return None
-    if w.dtype == torch.bfloat16:
-        return matmul_fp8_block(a_t, b_t)
-    return matmul_fp8_block(a_t, b_t, out_dtype=torch.float32).to(w.dtype)
+    if main is not None and main.dtype == torch.float32 and main.is_contiguous():
+        return main, _ADD
+    out = torch.empty(w.shape, dtype=torch.bfloat16 if w.dtype == torch.bfloat16 and main is None else torch.float32,
+                      device=w.device)
+    return out, _mode(out.dtype)
+
+
+def _returned(w, out):
+    """What autograd gets for ``w`` once ``_gradient_of``'s tensor is written."""
+    main = main_grad_of(w)
+    if main is None:
+        return out.to(w.dtype)
+    if out is not main:
+        main.add_(out)
+    return None
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_bytes(T, K, N, need, y_mode, dw_mode):
+    out = (_L * 3)()
+    _fn("lb_linear_block_bytes")(T, K, N, need, y_mode, dw_mode, ctypes.addressof(out))
+    return tuple(out)
+
+
+@functools.lru_cache(maxsize=4096)
+def _linear_kept_bytes(T, K, N, y_mode):
+    return _fn("lb_linear_kept_bytes")(T, K, N, y_mode)
+
+
+def _check_widths(*widths):
+    if any(n % 8 for n in widths):
+        raise ValueError(f"block-scaled layers need multiples of 8 features, got {widths}")
 
 
 class _LinearFp8Block(torch.autograd.Function):
+    """On the GPU: one native call each way. ``saved`` holds the transposed 8-bit copies of x and w, all that the
+    backward reads of them."""
+
     @staticmethod
     def forward(ctx, x, w, bias):
         x2 = x.reshape(-1, x.shape[-1])
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        xq, xq_t = quantize_fp8_block(x2, want_t=need_w)
-        wq, wq_t = quantize_fp8_block(w, tile=True, want_t=need_x)
-        ctx.shape, ctx.tokens, ctx.features = x.shape, x2.shape[0], w.shape
-        ctx.act_dtype = x.dtype if x.dtype in (torch.bfloat16, torch.float32) else torch.bfloat16
-        ctx.x_dtype, ctx.bias_dtype = x.dtype, None if bias is None else bias.dtype
-        # the backward pass needs only the transposed 8-bit copies (and the weight as an address)
-        ctx.save_for_backward(*((xq_t.data, xq_t.scales) if need_w else (None, None)),
-                              *((wq_t.data, wq_t.scales) if need_x else (None, None)), w)
-        y = matmul_fp8_block(xq, wq, out_dtype=ctx.act_dtype, bias=bias)
-        return y.view(*x.shape[:-1], w.shape[0])
+        T, K = x2.shape
+        N = w.shape[0]
+        ctx.need = need = ctx.needs_input_grad[0] + 2 * ctx.needs_input_grad[1] + 4 * ctx.needs_input_grad[2]
+        ctx.x_like = (x.shape, x.dtype)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        act = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
+        if not nv.use_native(x, w, bias):
+            xq, xq_t = _quantize_eager(x2, False, False, True, True)
+            wq, _ = _quantize_eager(w, True, False, True, False)
+            ctx.save_for_backward(w, xq_t.dequantize(), wq.dequantize())
+            return matmul_fp8_block(xq, wq, out_dtype=act, bias=bias).view(*x.shape[:-1], N)
+        _check_widths(K, N)
+        with _on_device(x, w, bias):
+            x2, w2 = _aligned(x2), _aligned(w)
+            if bias is not None:
+                bias = bias.to(torch.bfloat16).contiguous()
+            n_saved, n_tmp, _ = _linear_bytes(T, K, N, need, _mode(act), _BF16)
+            saved, tmp = _bytes(n_saved, x.device), _bytes(n_tmp, x.device)
+            y = torch.empty(*x.shape[:-1], N, dtype=act, device=x.device)
+            _call("lb_linear_block_fwd", x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), nv.ptr(bias), T, K, N,
+                  need, _mode(act), y.data_ptr(), saved.data_ptr(), tmp.data_ptr(),
+                  nv.status_word(x.device).data_ptr(), nv.stream_ptr())
+            nv.count_launch(3)
+        ctx.save_for_backward(w, saved)
+        return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
-        xt, xs, wt, ws, w = ctx.saved_tensors
-        dy2 = dy.reshape(-1, dy.shape[-1])
+        w = ctx.saved_tensors[0]
+        shape, x_dtype = ctx.x_like
+        N, K = w.shape
+        dy2 = dy.reshape(-1, N)
+        T, need = dy2.shape[0], ctx.need
         dx = dw = db = None
-        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        if need_x or need_w:
-            dyq, dyq_t = quantize_fp8_block(dy2, want=need_x, want_t=need_w)
-        if need_x:
-            dx = matmul_fp8_block(dyq, Fp8BlockTensor(wt, ctx.features[0], ws), out_dtype=ctx.act_dtype)
-            dx = dx.view(ctx.shape).to(ctx.x_dtype)
-        if need_w:
-            dw = _weight_gradient(w, dyq_t, Fp8BlockTensor(xt, ctx.tokens, xs))
-        if ctx.bias_dtype is not None and ctx.needs_input_grad[2]:
-            db = dy2.float().sum(0).to(ctx.bias_dtype)
-        return dx, dw, db
+        if len(ctx.saved_tensors) == 3:      # on the CPU
+            _, xv_t, wv = ctx.saved_tensors
+            dq, dq_t = _quantize_eager(dy2, False, False, True, True)
+            if need & 1:
+                dx = (dq.dequantize() @ wv).view(shape).to(x_dtype)
+            if need & 2:
+                dw = (dq_t.dequantize() @ xv_t.t()).to(w.dtype)
+            if need & 4:
+                db = dy2.float().sum(0).to(ctx.bias_dtype)
+            return dx, dw, db
+        saved = ctx.saved_tensors[1]
+        with _on_device(dy, w):
+            dy2 = _aligned(dy2)
+            if need & 1:
+                dx = torch.empty(shape, dtype=torch.float32 if x_dtype == torch.float32 else torch.bfloat16,
+                                 device=dy.device)
+            g = _gradient_of(w) if need & 2 else (None, _BF16)
+            if need & 4:
+                db = torch.empty(N, dtype=torch.bfloat16 if ctx.bias_dtype == torch.bfloat16 else torch.float32,
+                                 device=dy.device)
+            x_mode = _FP32 if dx is not None and dx.dtype == torch.float32 else _BF16
+            tmp = _bytes(_linear_bytes(T, K, N, need, x_mode, g[1])[2], dy.device)
+            _call("lb_linear_block_bwd", dy2.data_ptr(), dy2.stride(0), T, K, N, need, saved.data_ptr(), tmp.data_ptr(),
+                  nv.ptr(dx), x_mode, nv.ptr(g[0]), g[1], nv.ptr(db), 0 if db is None else _mode(db.dtype),
+                  nv.status_word(dy.device).data_ptr(), nv.stream_ptr())
+            nv.count_launch(1 + bool(need & 1) + bool(need & 2) + bool(need & 4))
+            dw = _returned(w, g[0]) if need & 2 else None
+            return (None if dx is None else dx.to(x_dtype)), dw, (None if db is None else db.to(ctx.bias_dtype))
 
 
 def linear_fp8_block(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -341,33 +431,40 @@ def linear_fp8_block(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) ->
     ``N`` are multiples of 8. The weight gradient goes into the fp32 accumulator of the sharding runtime
     where the weight has one.
     """
-    if w.shape[1] != x.shape[-1]:
-        raise ValueError(f"x has {x.shape[-1]} features and w takes {w.shape[1]}")
-    if isinstance(w, Fp8BlockTensor):
-        if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
-            raise ValueError("a kept 8-bit weight is for passes without gradients")
-        xq, _ = quantize_fp8_block(x.reshape(-1, x.shape[-1]))
-        y = matmul_fp8_block(xq, w, out_dtype=x.dtype if x.dtype == torch.float32 else torch.bfloat16, bias=bias)
-        return y.view(*x.shape[:-1], w.rows)
-    return _LinearFp8Block.apply(x, w, bias)
+    N, K = w.shape
+    if K != x.shape[-1]:
+        raise ValueError(f"x has {x.shape[-1]} features and w takes {K}")
+    if bias is not None and tuple(bias.shape) != (N,):
+        raise ValueError(f"bias has to be [{N}]")
+    if not isinstance(w, Fp8BlockTensor):
+        if x.numel() == 0 or N == 0:
+            return torch.nn.functional.linear(x, w.to(x.dtype), None if bias is None else bias.to(x.dtype))
+        if not torch.is_grad_enabled():      # nothing is kept for a backward then
+            x, w, bias = x.detach(), w.detach(), None if bias is None else bias.detach()
+        return _LinearFp8Block.apply(x, w, bias)
+    w.check("w")
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise ValueError("a kept 8-bit weight is for passes without gradients")
+    act = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
+    x2 = x.reshape(-1, K)
+    if x2.numel() == 0 or N == 0 or not nv.use_native(x, w.data, bias):
+        xq, _ = quantize_fp8_block(x2)
+        return matmul_fp8_block(xq, w, out_dtype=act, bias=bias).view(*x.shape[:-1], N)
+    _check_widths(K, N)
+    with _on_device(x, w.data, bias):
+        x2 = _aligned(x2)
+        if bias is not None:
+            bias = bias.to(torch.bfloat16).contiguous()
+        T, mode = x2.shape[0], _mode(act)
+        y = torch.empty(*x.shape[:-1], N, dtype=act, device=x.device)
+        tmp = _bytes(_linear_kept_bytes(T, K, N, mode), x.device)
+        _call("lb_linear_kept_fwd", x2.data_ptr(), x2.stride(0), *_where(w), w.e5m2, nv.ptr(bias), T, K, N, mode,
+              y.data_ptr(), tmp.data_ptr(), nv.status_word(x.device).data_ptr(), nv.stream_ptr())
+        nv.count_launch(2)
+    return y
 
 
 _KINDS = {"swiglu": 0, "geglu": 1}
-
-
-def _glu_forward(gu, kind) -> Fp8BlockTensor:
-    """``act(gate) * up`` (bf16 values) of ``gu = [gate | up]``, cast in blocks of a row."""
-    T, I = gu.shape[0], gu.shape[1] // 2
-    if not nv.use_native(gu):
-        return _quantize_eager(glu_ref(gu[:, :I], gu[:, I:], kind), False, False, True, False)[0]
-    h = _empty(T, I, False, gu.device)
-    if T:
-        rc = _fn("lb_block_glu_fwd")(_KINDS[kind], gu.data_ptr(), gu.data_ptr() + 2 * I, gu.stride(0), T, I, *_where(h),
-                                     nv.stream_ptr())
-        if rc != 0:
-            nv.check_rc(rc, f"lb_block_glu_fwd(T={T},I={I})")
-        nv.count_launch()
-    return h
 
 
 def _glu_grad_ref(g, u, dh, kind):
@@ -382,96 +479,103 @@ def _glu_grad_ref(g, u, dh, kind):
     return torch.cat([dh * u * da, dh * a], dim=1).to(torch.bfloat16)
 
 
-def _glu_backward(dh, gu, kind, want, want_t, want_h):
-    """Gradients of ``gu`` in blocks of a row and of 128 tokens, and ``h`` in blocks of 128 tokens."""
-    T, I = gu.shape[0], gu.shape[1] // 2
-    if not nv.use_native(dh):
-        d, d_t = _quantize_eager(_glu_grad_ref(gu[:, :I], gu[:, I:], dh, kind), False, False, want, want_t)
-        h_t = _quantize_eager(glu_ref(gu[:, :I], gu[:, I:], kind), False, False, False, True)[1] if want_h else None
-        return d, d_t, h_t
-    d = _empty(T, 2 * I, False, gu.device) if want else None
-    d_t = _empty(2 * I, T, False, gu.device) if want_t else None
-    h_t = _empty(I, T, False, gu.device) if want_h else None
-    if T:
-        rc = _fn("lb_block_glu_bwd")(_KINDS[kind], dh.data_ptr(), dh.stride(0), gu.data_ptr(), gu.data_ptr() + 2 * I,
-                                     gu.stride(0), T, I, *_where(d), *_where(d_t), *_where(h_t), nv.stream_ptr())
-        if rc != 0:
-            nv.check_rc(rc, f"lb_block_glu_bwd(T={T},I={I})")
-        nv.count_launch()
-    return d, d_t, h_t
-
-
-def _cast_pair(w_gate, w_up, want_t):
-    """Gate and up weights as one block-scaled ``[2 I, K]`` matrix (and its transpose), wherever they lie."""
-    if w_up is None:
-        return quantize_fp8_block(w_gate, tile=True, want_t=want_t)
-    if not nv.use_native(w_gate, w_up):
-        return _quantize_eager(torch.cat([w_gate, w_up]), True, False, True, want_t)
-    I, K = w_gate.shape
-    if K % 8:
-        raise ValueError("quantize_fp8_block needs a multiple of 8 columns")
-    q = _empty(2 * I, K, False, w_gate.device)
-    q_t = _empty(K, 2 * I, False, w_gate.device) if want_t else None
-    for lo, w in ((0, _aligned(w_gate.detach())), (I, _aligned(w_up.detach()))):
-        part = Fp8BlockTensor(q.data[lo:lo + I], K, q.scales[:, lo:lo + I])
-        part_t = (0, 0, 0, 0)
-        if want_t:
-            part_t = (q_t.data.data_ptr() + lo, _row_bytes(q_t.data), q_t.scales.data_ptr(), K)
-        rc = _fn("lb_block_cast")(w.data_ptr(), I, K, w.stride(0), True, False, *_where(part), *part_t, lo // BLOCK,
-                                  nv.stream_ptr())
-        if rc != 0:
-            nv.check_rc(rc, f"lb_block_cast(R={I},C={K})")
-    nv.count_launch(2)
-    return q, q_t
-
-
-def _mlp_forward(xq, w, wd, kind):
-    """Gate and up products (bf16) and the block's output."""
+def _mlp_eager(xq, w, wd, kind):
+    """Gate and up products, ``h`` (both bf16 values) and the output."""
     gu = matmul_fp8_block(xq, w)
-    return gu, matmul_fp8_block(_glu_forward(gu, kind), wd)
+    I = gu.shape[1] // 2
+    h = glu_ref(gu[:, :I], gu[:, I:], kind)
+    return gu, h, matmul_fp8_block(_quantize_eager(h, False, False, True, False)[0], wd)
+
+
+@functools.lru_cache(maxsize=4096)
+def _mlp_bytes(T, H, I, need, *modes):
+    out, m = (_L * 3)(), (_I * 3)(*modes)
+    _fn("lb_mlp_block_bytes")(T, H, I, need, ctypes.addressof(m), ctypes.addressof(out))
+    return tuple(out)
+
+
+@functools.lru_cache(maxsize=4096)
+def _mlp_kept_bytes(T, H, I):
+    return _fn("lb_mlp_kept_bytes")(T, H, I)
 
 
 class _GatedMlpFp8Block(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, w_gate, w_up, w_down, kind):
-        x2 = x.reshape(-1, x.shape[-1])
-        need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
-        need_gu = need_g or need_u
-        xq, xq_t = quantize_fp8_block(x2, want_t=need_gu)
-        wq, wq_t = _cast_pair(w_gate, w_up, need_x)
-        dq, dq_t = quantize_fp8_block(w_down, tile=True, want_t=need_x or need_gu)
-        gu, y = _mlp_forward(xq, wq, dq, kind)
-        ctx.save_for_backward(gu, *(t for q in (xq_t, wq_t, dq_t) for t in ((q.data, q.scales) if q else (None, None))),
-                              w_gate, w_up, w_down)
-        ctx.kind, ctx.shape, ctx.dtype = kind, x.shape, x.dtype
-        return y.view(x.shape).to(x.dtype if x.dtype == torch.float32 else torch.bfloat16)
+    """On the GPU: one native call each way. ``saved`` holds gate and up products and the transposed 8-bit copies of x and
+    the weights."""
 
     @staticmethod
+    def forward(ctx, x, w_gate, w_up, w_down, kind):
+        H, I = w_down.shape
+        x2 = x.reshape(-1, H)
+        T = x2.shape[0]
+        nx, ng, nu, nd = ctx.needs_input_grad[:4]
+        ctx.need = need = nx + 2 * (ng or nu) + 4 * nd
+        ctx.kind, ctx.x_like = kind, (x.shape, x.dtype)
+        act = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
+        if not nv.use_native(x, w_gate, w_up, w_down):
+            xq, xq_t = _quantize_eager(x2, False, False, True, True)
+            w = w_gate if w_up is None else torch.cat([w_gate, w_up])
+            wq, dq = (_quantize_eager(t, True, False, True, False)[0] for t in (w, w_down))
+            gu, h, y = _mlp_eager(xq, wq, dq, kind)
+            ctx.save_for_backward(w_gate, w_up, w_down, gu, h, xq_t.dequantize(), wq.dequantize(), dq.dequantize())
+            return y.view(x.shape).to(act)
+        _check_widths(H)
+        with _on_device(x, w_gate, w_up, w_down):
+            x2, wg, wd = _aligned(x2), _aligned(w_gate), _aligned(w_down)
+            wu = None if w_up is None else _aligned(w_up)
+            n_saved, n_tmp, _ = _mlp_bytes(T, H, I, need, 0, 0, 0)
+            saved, tmp = _bytes(n_saved, x.device), _bytes(n_tmp, x.device)
+            y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+            _call("lb_mlp_block_fwd", _KINDS[kind], x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), nv.ptr(wu),
+                  0 if wu is None else wu.stride(0), wd.data_ptr(), wd.stride(0), T, H, I, need, y.data_ptr(),
+                  saved.data_ptr(), tmp.data_ptr(), nv.status_word(x.device).data_ptr(), nv.stream_ptr())
+            nv.count_launch(5 + (wu is not None))
+        ctx.save_for_backward(w_gate, w_up, w_down, saved)
+        return y.to(act)
+
+    @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
-        gu, xt, xs, wt, ws, dt, ds, w_gate, w_up, w_down = ctx.saved_tensors
-        need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
-        need_gu = need_g or need_u
-        T, I = gu.shape[0], gu.shape[1] // 2
+        w_gate, w_up, w_down = ctx.saved_tensors[:3]
+        shape, x_dtype = ctx.x_like
+        H, I = w_down.shape
+        dy2 = dy.reshape(-1, H)
+        T, need = dy2.shape[0], ctx.need
+        nx, ng, nu, nd = ctx.needs_input_grad[:4]
         dx = dg = du = dd = None
-        dyq, dyq_t = quantize_fp8_block(dy.reshape(T, -1), want=need_x or need_gu, want_t=need_d)
-        if need_x or need_gu:
-            dh = matmul_fp8_block(dyq, Fp8BlockTensor(dt, w_down.shape[0], ds))
-        else:
-            dh = gu[:, :I]      # not read for h
-        d, d_t, h_t = _glu_backward(dh, gu, ctx.kind, need_x, need_gu, need_d)
-        if need_x:
-            dx = matmul_fp8_block(d, Fp8BlockTensor(wt, 2 * I, ws)).view(ctx.shape).to(ctx.dtype)
-        if need_gu:
-            x_t = Fp8BlockTensor(xt, T, xs)
-            if w_up is None:
-                dg = _weight_gradient(w_gate, d_t, x_t)
-            else:
-                half = lambda lo: Fp8BlockTensor(d_t.data[lo:lo + I], T, d_t.scales[:, lo:lo + I])  # noqa: E731
-                dg = _weight_gradient(w_gate, half(0), x_t) if need_g else None
-                du = _weight_gradient(w_up, half(I), x_t) if need_u else None
-        if need_d:
-            dd = _weight_gradient(w_down, dyq_t, h_t)
-        return dx, dg, du, dd, None
+        if len(ctx.saved_tensors) > 4:       # on the CPU
+            gu, h, xv_t, wv, dv = ctx.saved_tensors[3:]
+            dq, dq_t = _quantize_eager(dy2, False, False, True, True)
+            dh = (dq.dequantize() @ dv).to(torch.bfloat16)
+            d, d_t = _quantize_eager(_glu_grad_ref(gu[:, :I], gu[:, I:], dh, ctx.kind), False, False, True, True)
+            if nx:
+                dx = (d.dequantize() @ wv).to(torch.bfloat16).view(shape).to(x_dtype)
+            if need & 2:
+                dw = d_t.dequantize() @ xv_t.t()
+                if w_up is None:
+                    dg = dw.to(w_gate.dtype)
+                else:
+                    dg, du = (t.to(w_gate.dtype) if n else None for t, n in ((dw[:I], ng), (dw[I:], nu)))
+            if nd:
+                h_t = _quantize_eager(h, False, False, False, True)[1].dequantize()
+                dd = (dq_t.dequantize() @ h_t.t()).to(w_down.dtype)
+            return dx, dg, du, dd, None
+        saved = ctx.saved_tensors[3]
+        with _on_device(dy, w_down):
+            dy2 = _aligned(dy2)
+            dx = torch.empty(shape, dtype=torch.bfloat16, device=dy.device) if nx else None
+            grads = [_gradient_of(w) if n else (None, _BF16)
+                     for w, n in ((w_gate, ng), (w_up, nu), (w_down, nd))]
+            modes = [g[1] for g in grads]
+            tmp = _bytes(_mlp_bytes(T, H, I, need, *modes)[2], dy.device)
+            m = (_I * 3)(*modes)
+            _call("lb_mlp_block_bwd", _KINDS[ctx.kind], dy2.data_ptr(), dy2.stride(0), T, H, I, need, w_up is None,
+                  saved.data_ptr(), tmp.data_ptr(), nv.ptr(dx), *(nv.ptr(g[0]) for g in grads), ctypes.addressof(m),
+                  nv.status_word(dy.device).data_ptr(), nv.stream_ptr())
+            nv.count_launch(2 + bool(need & 3) + nx + ng + nu + nd)
+            dg, du, dd = (_returned(w, g[0]) if n else None
+                          for w, n, g in zip((w_gate, w_up, w_down), (ng, nu, nd), grads))
+            return (None if dx is None else dx.to(x_dtype)), dg, du, dd, None
 
 
 def gated_mlp_fp8_block(x: torch.Tensor, w_gate, w_up, w_down, kind: str = "swiglu") -> torch.Tensor:
@@ -484,7 +588,7 @@ def gated_mlp_fp8_block(x: torch.Tensor, w_gate, w_up, w_down, kind: str = "swig
     ``quantize_fp8_block(w, tile=True)`` gives, all of them, with a fused gate and up weight.
 
     Gate and up products, ``act(gate) * up`` and its gradient, and the gradients of gate and up are rounded to
-    bf16, as they are between separate layers, before they are cast.
+    bf16, as they are between separate layers, before they are cast; so are ``y`` and ``dx``, whatever ``x``'s type.
     """
     if kind not in _KINDS:
         raise ValueError(f"unknown activation {kind!r}; choose from {tuple(_KINDS)}")
@@ -495,15 +599,37 @@ def gated_mlp_fp8_block(x: torch.Tensor, w_gate, w_up, w_down, kind: str = "swig
             raise ValueError(f"gate and up weights {tuple(w.shape)} do not fit w_down {tuple(w_down.shape)}")
     if x.shape[-1] != H:
         raise ValueError(f"x has {x.shape[-1]} features and the weights take {H}")
-    if I % BLOCK:
+    if I % BLOCK or I == 0:
         raise ValueError(f"the inner width has to be a multiple of {BLOCK}, got {I}")
     kept = [isinstance(w, Fp8BlockTensor) for w in (w_gate, w_up, w_down)]
-    if any(kept):
-        if not (kept[0] and kept[2]) or w_up is not None:
-            raise ValueError("8-bit weights come as a fused gate and up weight and a down weight")
-        if torch.is_grad_enabled() and x.requires_grad:
-            raise ValueError("a kept 8-bit weight is for passes without gradients")
-        xq, _ = quantize_fp8_block(x.reshape(-1, H))
-        y = _mlp_forward(xq, w_gate, w_down, kind)[1].view(x.shape)
-        return y.to(x.dtype) if x.dtype == torch.float32 else y
-    return _GatedMlpFp8Block.apply(x, w_gate, w_up, w_down, kind)
+    if not any(kept):
+        if x.numel() == 0:
+            zero = sum(w.sum() for w in (w_gate, w_up, w_down) if w is not None) * 0
+            return x * zero.to(x.dtype)      # keeps the graph: gradients of zero
+        if not torch.is_grad_enabled():      # nothing is kept for a backward then
+            x, w_gate, w_up, w_down = (t if t is None else t.detach() for t in (x, w_gate, w_up, w_down))
+        return _GatedMlpFp8Block.apply(x, w_gate, w_up, w_down, kind)
+    if not (kept[0] and kept[2]) or w_up is not None:
+        raise ValueError("8-bit weights come as a fused gate and up weight and a down weight")
+    w_gate.check("w_gate")
+    w_down.check("w_down")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("a kept 8-bit weight is for passes without gradients")
+    act = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
+    if x.numel() == 0:
+        return torch.empty(x.shape, dtype=act, device=x.device)
+    x2 = x.reshape(-1, H)
+    if not nv.use_native(x, w_gate.data, w_down.data):
+        xq, _ = _quantize_eager(x2, False, False, True, False)
+        return _mlp_eager(xq, w_gate, w_down, kind)[2].view(x.shape).to(act)
+    _check_widths(H)
+    with _on_device(x, w_gate.data, w_down.data):
+        x2 = _aligned(x2)
+        T = x2.shape[0]
+        y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
+        tmp = _bytes(_mlp_kept_bytes(T, H, I), x.device)
+        _call("lb_mlp_kept_fwd", _KINDS[kind], x2.data_ptr(), x2.stride(0), *_where(w_gate), w_gate.e5m2,
+              *_where(w_down), w_down.e5m2, T, H, I, y.data_ptr(), tmp.data_ptr(),
+              nv.status_word(x.device).data_ptr(), nv.stream_ptr())
+        nv.count_launch(4)
+    return y.to(act)

@@ -67,7 +67,10 @@ def test_cast_of_strided_and_unaligned_inputs():
 
 SHAPES = [(1, 128, 128), (1, 8, 16), (5, 264, 272), (16, 128, 1024), (17, 136, 520), (33, 1000, 640), (64, 256, 4096),
           (65, 512, 2560), (128, 128, 128), (129, 257, 144), (300, 264, 208), (500, 384, 1920), (1, 2560, 9728),
-          (12, 4096, 2560), (1000, 1032, 1040)]
+          (12, 4096, 2560), (1000, 1032, 1040),
+          # tiles of CTA pairs: one stage, whole and ragged ones, more tiles than pairs, bands of them
+          (1030, 2304, 16), (1500, 2056, 256), (2000, 2304, 640), (2561, 1288, 1040), (4097, 4360, 2576),
+          (1100, 16392, 2064)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
@@ -82,7 +85,7 @@ def test_product(M, N, K, tile):
         _check_product(c, a, b)
 
 
-@pytest.mark.parametrize("M,N,K", [(5, 264, 272), (200, 384, 1040)])
+@pytest.mark.parametrize("M,N,K", [(5, 264, 272), (200, 384, 1040), (1800, 1800, 640)])
 @pytest.mark.parametrize("formats", [(True, False), (False, True), (True, True)])
 def test_product_of_either_format(M, N, K, formats):
     a, _ = fb.quantize_fp8_block(_rand(M, K), e5m2=formats[0])
@@ -90,7 +93,7 @@ def test_product_of_either_format(M, N, K, formats):
     _check_product(fb.matmul_fp8_block(a, b, out_dtype=torch.float32), a, b)
 
 
-@pytest.mark.parametrize("M,N,K", [(3, 136, 640), (150, 256, 272), (700, 520, 1040)])
+@pytest.mark.parametrize("M,N,K", [(3, 136, 640), (150, 256, 272), (700, 520, 1040), (1700, 1800, 1040)])
 def test_bias_accumulation_and_outputs_within_a_larger_tensor(M, N, K):
     a, _ = fb.quantize_fp8_block(_rand(M, K))
     b, _ = fb.quantize_fp8_block(_rand(N, K, seed=1), tile=True)
@@ -169,7 +172,7 @@ def _off(a, b):
     return float((a.double() - b).norm() / b.norm().clamp(min=1e-300))
 
 
-TOKENS = [1, 2, 15, 64, 129, 333, 1000]
+TOKENS = [1, 2, 15, 64, 129, 333, 1000, 2600]
 
 
 @pytest.mark.parametrize("T", TOKENS)
@@ -210,26 +213,30 @@ def test_weight_gradients_go_to_the_accumulator():
     assert w.grad is None and _off(w.main_grad - 3, want) < 1e-5
 
 
+# Sizes at which the products of both ways run in the same kernel, unsplit: the sums' order is the same.
 @pytest.mark.parametrize("kind", ["swiglu", "geglu"])
-@pytest.mark.parametrize("T,I", [(1, 128), (100, 384), (128, 256), (259, 640)])
-def test_cast_activations_have_the_bytes_of_the_separate_steps(T, I, kind):
+@pytest.mark.parametrize("T,H,I", [(1, 256, 128), (100, 264, 384), (2049, 2048, 1280), (1500, 4104, 1024)])
+def test_gated_mlp_has_the_bits_of_the_separate_steps(T, H, I, kind):
     from lset_b200.ops.activation import glu
 
-    gu, dh = _rand(T, 2 * I, spread=1.0).requires_grad_(), _rand(T, I, seed=1, spread=1.0)
+    x, dy = _rand(T, H, spread=0.5), _rand(T, H, seed=1, spread=1.0)
+    w, wd = (_rand(2 * I, H, seed=2, spread=0.3) * H ** -0.5), (_rand(H, I, seed=3, spread=0.3) * I ** -0.5)
+    leaves = [t.requires_grad_() for t in (x, w, wd)]
+    y = fb.gated_mlp_fp8_block(x, w, None, wd, kind)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    with torch.no_grad():
+        (xq, xt), (dq, dt) = fb.quantize_fp8_block(x, want_t=True), fb.quantize_fp8_block(dy, want_t=True)
+        (wq, wt), (vq, vt) = (fb.quantize_fp8_block(t, tile=True, want_t=True) for t in (w, wd))
+        gu, dh = fb.matmul_fp8_block(xq, wq), fb.matmul_fp8_block(dq, vt)
+    gu.requires_grad_()
     h = glu(gu, kind)
     (dgu,) = torch.autograd.grad(h, gu, dh)
-    gu, h = gu.detach(), h.detach()
-    with torch.no_grad():
-        _same_bytes(fb._glu_forward(gu, kind), _cpu(fb.quantize_fp8_block(h)[0]))
-        d, d_t, h_t = fb._glu_backward(dh, gu, kind, True, True, True)
-        want, want_t = fb.quantize_fp8_block(dgu, want_t=True)
-        _same_bytes(d, _cpu(want))
-        _same_bytes(d_t, _cpu(want_t))
-        _same_bytes(h_t, _cpu(fb.quantize_fp8_block(h, want=False, want_t=True)[1]))
-
-
-def _cpu(q):
-    return fb.Fp8BlockTensor(q.data.cpu(), q.cols, q.scales.cpu(), q.e5m2)
+    (hq, ht), (d, d_t) = fb.quantize_fp8_block(h, want_t=True), fb.quantize_fp8_block(dgu, want_t=True)
+    want = [fb.matmul_fp8_block(hq, vq), fb.matmul_fp8_block(d, wt), fb.matmul_fp8_block(d_t, xt),
+            fb.matmul_fp8_block(dt, ht)]
+    nv.check_status()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
 
 
 def _mlp_want(x, wgu, wd, kind, dy):
