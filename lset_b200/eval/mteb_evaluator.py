@@ -40,7 +40,9 @@ class LSETMTEBModel:
 
     @classmethod
     def from_pretrained(cls, model_path: str, pooling: str = "auto", max_length: int = 512,
-                        device: Optional[str] = None, dtype=None, **kw) -> "LSETMTEBModel":
+                        device: Optional[str] = None, dtype=None, fp8: bool = False,
+                        **kw) -> "LSETMTEBModel":
+        """``fp8``: the linear layers keep block-scaled 8-bit weights."""
         from ..tokenization import load_tokenizer
 
         name = detect_model_type(model_path)
@@ -51,6 +53,10 @@ class LSETMTEBModel:
         dev = torch.device(device or ("cuda" if torch.cuda.is_available() else "cpu"))
         dtype = dtype or (torch.bfloat16 if dev.type == "cuda" else torch.float32)
         model = model.to(device=dev, dtype=dtype)
+        if fp8:
+            from ..train.quantization.fp8 import apply_fp8_inference
+
+            apply_fp8_inference(model)
         pool = spec.default_pooling if pooling in (None, "auto") else pooling
         proj = spec.post_pooling_fn(model_path) if spec.post_pooling_fn is not None else None
         if proj is not None:

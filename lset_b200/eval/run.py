@@ -11,8 +11,10 @@ def run_eval(config: LSETConfig):
         raise SystemExit("evaluation needs the optional dependency `mteb` (pip install mteb>=2)") from exc
     from .mteb_evaluator import LSETMTEBModel
 
+    # a model trained with block-scaled products is evaluated with them, on 8-bit weights
+    fp8 = {"fp8": True} if config.fp8.enabled and config.fp8.recipe == "block128" else {}
     model = LSETMTEBModel.from_pretrained(resolve_path(config.model.path), pooling=config.model.pooling,
-                                          max_length=config.eval.max_length)
+                                          max_length=config.eval.max_length, **fp8)
     names = config.eval.tasks or ["STSBenchmark"]
     tasks = mteb.get_tasks(tasks=names)
     results = mteb.evaluate(model, tasks, encode_kwargs={"batch_size": config.eval.batch_size})

@@ -19,9 +19,11 @@ import torch.nn as nn
 from ..ops import activation as act_ops
 from ..ops import attention as attn_ops
 from ..ops import embedding as emb_ops
+from ..ops import fp8_block as fp8_block_ops
 from ..ops import gemm as gemm_ops
 from ..ops import norm as norm_ops
 from ..ops import rope as rope_ops
+from ..ops.block import unhooked
 from ..ops.runtime_options import enabled
 
 
@@ -176,7 +178,30 @@ class GatedMLP(nn.Module):
             self.up_proj = Linear(hidden_size, intermediate_size, bias=False)
         self.down_proj = Linear(intermediate_size, hidden_size, bias=False)
 
+    def _fp8_block_weights(self):
+        """(gate or fused, up or None, down) where all projections have block-scaled 8-bit weights and nothing of
+        their own around the product (hooks, a tensor-parallel forward), and the operator takes their widths."""
+        mods = ([self.gate_up_proj] if self.fused_gate_up else [self.gate_proj, self.up_proj]) + [self.down_proj]
+        out = []
+        for m in mods:
+            weight = getattr(m, "fp8_block_weight", None)
+            weight = weight() if weight is not None and m.bias is None and unhooked(m.__dict__) else None
+            if weight is None:
+                return None
+            out.append(weight)
+        if out[-1].shape[1] % fp8_block_ops.BLOCK or any(type(w) is not type(out[0]) for w in out):
+            return None
+        if self.fused_gate_up:
+            out.insert(1, None)
+        elif isinstance(out[0], fp8_block_ops.Fp8BlockTensor):
+            return None
+        return out
+
     def forward(self, x):
+        if getattr(self.down_proj, "fp8_block_weight", None) is not None:
+            weights = self._fp8_block_weights()
+            if weights is not None:
+                return fp8_block_ops.gated_mlp_fp8_block(x, *weights, self.kind)
         if self.fused_gate_up:
             gu = self.gate_up_proj
             # plain bf16 projection on the GPU: the activation rides in the GEMM epilogue; wrapped

@@ -15,10 +15,18 @@ scaling — e4m3 for activations and weights, e5m2 for output gradients:
     feature (both over the tokens).
 ``rowwise_with_gw_hp``
     as ``rowwise`` but the weight gradient is computed from the bf16 tensors.
+``block128``
+    one power-of-two scale for each 128 values along the contraction (activations, output gradients, both
+    e4m3) or 128 x 128 tile (weights): an outlier costs its own block range, not its tensor or row
+    (``ops/fp8_block.py``, scales applied by the tensor cores). A ``GatedMLP`` of such layers runs as one
+    operator, whose activations are cast where they are computed.
 
 Weight gradients go straight into the fp32 accumulator of the sharding runtime when the weight has
 one. On the CPU the same quantise → multiply → rescale arithmetic runs in plain PyTorch.
 ``get_fp8_tp_plan`` mirrors the reference's plan helper.
+
+``apply_fp8_inference(model)`` is for models that only encode: their linear layers keep block-scaled 8-bit
+weights (half the memory of bf16, nothing to cast but the activations).
 """
 from __future__ import annotations
 
@@ -28,10 +36,11 @@ import torch
 import torch.nn as nn
 
 from ...ops import fp8 as f8
+from ...ops import fp8_block as fb
 from ...ops._grads import main_grad_of
 from ...ops.gemm import _accumulate_wgrad, wgrad_splits
 
-RECIPES = ("tensorwise", "rowwise", "rowwise_with_gw_hp")
+RECIPES = ("tensorwise", "rowwise", "rowwise_with_gw_hp", "block128")
 E4M3_MAX, E5M2_MAX = f8.E4M3_MAX, f8.E5M2_MAX
 
 
@@ -112,9 +121,15 @@ class _Fp8Linear(torch.autograd.Function):
 class Float8Linear(nn.Linear):
     recipe = "rowwise"
 
+    def fp8_block_weight(self):
+        """The weight as ``ops.fp8_block`` takes it, or None where this layer has no block scales."""
+        return self.weight if self.recipe == "block128" else None
+
     def forward(self, x):
         if x.numel() == 0:
             return torch.nn.functional.linear(x, self.weight, self.bias)
+        if self.recipe == "block128":
+            return fb.linear_fp8_block(x, self.weight, self.bias)
         return _Fp8Linear.apply(x, self.weight, self.bias, self.recipe != "tensorwise",
                                 self.recipe == "rowwise_with_gw_hp")
 
@@ -130,6 +145,46 @@ def apply_fp8_training(model: nn.Module, recipe: str = "rowwise") -> nn.Module:
         if isinstance(mod, nn.Linear) and _eligible(mod) and type(mod).__name__ in ("Linear",):
             mod.__class__ = Float8Linear
             mod.recipe = recipe
+    return model
+
+
+class Fp8KeptLinear(nn.Module):
+    """A linear layer for passes without gradients whose weight is kept in 8 bits, in 128 x 128 blocks."""
+
+    def __init__(self, weight: torch.Tensor, bias=None):
+        super().__init__()
+        self.out_features, self.in_features = weight.shape
+        q, _ = fb.quantize_fp8_block(weight.detach(), tile=True)
+        self.register_buffer("weight", q.data)        # bytes [out_features, ld]
+        self.register_buffer("scales", q.scales)
+        self.register_buffer("bias", None if bias is None else bias.detach().clone())
+
+    def fp8_block_weight(self):
+        return fb.Fp8BlockTensor(self.weight, self.in_features, self.scales)
+
+    def forward(self, x):
+        return fb.linear_fp8_block(x, self.fp8_block_weight(), self.bias)
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+def apply_fp8_inference(model: nn.Module) -> nn.Module:
+    """Replaces, in place, every eligible linear layer of a model that only encodes by an ``Fp8KeptLinear``. Separate
+    gate and up projections of a gated MLP become one fused layer, which the fused operator takes."""
+    from ...models.layers import GatedMLP
+
+    for mod in list(model.modules()):
+        if (isinstance(mod, GatedMLP) and not mod.fused_gate_up
+                and all(type(m).__name__ == "Linear" and _eligible(m) and m.bias is None
+                        for m in (mod.gate_proj, mod.up_proj))):
+            mod.gate_up_proj = Fp8KeptLinear(torch.cat([mod.gate_proj.weight, mod.up_proj.weight]))
+            mod.fused_gate_up = True
+            del mod.gate_proj, mod.up_proj
+    for mod in list(model.modules()):
+        for name, child in list(mod.named_children()):
+            if isinstance(child, nn.Linear) and type(child).__name__ == "Linear" and _eligible(child):
+                setattr(mod, name, Fp8KeptLinear(child.weight, child.bias))
     return model
 
 

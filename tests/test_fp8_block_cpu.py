@@ -260,3 +260,91 @@ def test_gated_mlp_refusals():
         fb.gated_mlp_fp8_block(x, q[0], None, wd)
     with pytest.raises(ValueError, match="without gradients"):
         fb.gated_mlp_fp8_block(x.requires_grad_(), q[0], None, q[1])
+
+
+# ------------------------------------------------------------------------------------------------
+# Models
+# ------------------------------------------------------------------------------------------------
+def _mlp(H, I, fused, recipe="block128"):
+    from lset_b200.models.layers import GatedMLP
+    from lset_b200.train.quantization.fp8 import apply_fp8_training
+
+    torch.manual_seed(11)
+    return apply_fp8_training(GatedMLP(H, I, "swiglu", fused), recipe)
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    seen = []
+    real = fb.gated_mlp_fp8_block
+    monkeypatch.setattr(fb, "gated_mlp_fp8_block", lambda *a: seen.append(a) or real(*a))
+    return seen
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_gated_mlp_module_runs_as_one_operator(fused, calls):
+    mlp = _mlp(64, 256, fused)
+    x = torch.randn(5, 64)
+    y = mlp(x)
+    assert len(calls) == 1
+    y.sum().backward()
+    assert all(p.grad is not None and p.grad.abs().sum() > 0 for p in mlp.parameters())
+    handle = mlp.down_proj.register_forward_hook(lambda *a: None)      # a hook wants the layer's own call
+    z = mlp(x)
+    assert len(calls) == 1 and torch.allclose(z, y, rtol=2e-2, atol=2e-2 * float(y.abs().max()))
+    handle.remove()
+    mlp.down_proj.forward = type(mlp.down_proj).forward.__get__(mlp.down_proj)   # and so does a replaced forward
+    mlp(x)
+    assert len(calls) == 1
+
+
+@pytest.mark.parametrize("H,I,recipe", [(64, 144, "block128"), (64, 256, "tensorwise")])
+def test_gated_mlp_module_of_other_widths_and_recipes_runs_layer_by_layer(H, I, recipe, calls):
+    y = _mlp(H, I, True, recipe)(torch.randn(5, H))
+    assert y.shape == (5, H) and not calls
+
+
+def _tiny():
+    from lset_b200.models import Qwen3Config, Qwen3Decoder
+
+    torch.manual_seed(12)
+    return Qwen3Decoder(Qwen3Config(vocab_size=97, hidden_size=64, intermediate_size=128, num_hidden_layers=2,
+                                    num_attention_heads=4, num_key_value_heads=2, head_dim=16)).eval()
+
+
+def test_inference_model_keeps_8_bit_weights(calls):
+    from lset_b200.train.quantization.fp8 import Fp8KeptLinear, apply_fp8_inference
+
+    model, ids = _tiny(), torch.randint(0, 97, (2, 9), generator=torch.Generator().manual_seed(0))
+    with torch.no_grad():
+        want = model(ids)["hidden_states"]
+        apply_fp8_inference(model)
+        got = model(ids)["hidden_states"]
+    kinds = [type(m) for m in model.modules()]
+    assert kinds.count(Fp8KeptLinear) == 2 * 6 and not any(issubclass(k, torch.nn.Linear) for k in kinds)
+    assert len(calls) == 2
+    # each of the seven products a layer is off by about 2^-4 / sqrt(3) x sqrt(2) relative to its norm at most
+    assert float(torch.nn.functional.cosine_similarity(got, want, dim=-1).min()) > 0.98
+    state = model.state_dict()
+    assert sum(v.dtype == torch.uint8 for v in state.values()) == 2 * 2 * 6
+    again = apply_fp8_inference(_tiny())
+    again.load_state_dict(state)
+    with torch.no_grad():
+        assert torch.equal(again(ids)["hidden_states"], got)
+
+
+def test_layers_of_biased_models_keep_their_bias():
+    from lset_b200.train.quantization.fp8 import Fp8KeptLinear, apply_fp8_inference
+
+    torch.manual_seed(13)
+    m = torch.nn.Sequential(torch.nn.Linear(64, 32), torch.nn.Linear(32, 20))
+    x = torch.randn(7, 64)
+    with torch.no_grad():
+        q, _ = fb.quantize_fp8_block(m[0].weight, tile=True)
+        want = fb.linear_fp8_block(x, q, m[0].bias)
+        last = m[1](want)
+        apply_fp8_inference(m)
+        assert isinstance(m[0], Fp8KeptLinear) and type(m[1]) is torch.nn.Linear     # 20: no multiple of 16
+        assert torch.equal(m[0](x), want) and torch.equal(m(x), last)
+    with pytest.raises(ValueError, match="without gradients"):
+        m[0](x.requires_grad_())

@@ -276,3 +276,136 @@ def test_gated_mlp_forward_and_gradients(T, H, I, kind):
     assert torch.equal(y2, y) and torch.equal(g2[0], got[1]) and torch.equal(g2[3], got[3])
     # (a product of half the rows may add its sums in another order: the same bound against the formula, then)
     assert _off(torch.cat([g2[1], g2[2]]), want[2]) < 2.0 ** -7
+
+
+# ------------------------------------------------------------------------------------------------
+# Ways of calling
+# ------------------------------------------------------------------------------------------------
+def test_no_result_depends_on_timing():
+    x, w = _rand(3000, 1040, spread=1.0).requires_grad_(), _rand(520, 1040, seed=1, spread=0.5).requires_grad_()
+    b, dy = _rand(520, seed=2, spread=0.5).requires_grad_(), _rand(3000, 520, seed=3, spread=1.0)
+    first = None
+    for _ in range(4):
+        out = torch.autograd.grad(fb.linear_fp8_block(x, w, b), (x, w, b), dy)
+        torch.cuda.synchronize()
+        first = first or out
+        assert all(torch.equal(a, c) for a, c in zip(first, out))
+
+
+def test_on_a_stream_of_its_own_and_from_two_threads():
+    import threading
+
+    x, w = _rand(700, 512, spread=1.0), _rand(1024, 512, seed=1, spread=0.5)
+    want = fb.linear_fp8_block(x, w)
+    torch.cuda.synchronize()
+    got = [None] * 4
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s), torch.no_grad():
+            for _ in range(10):
+                got[i] = fb.linear_fp8_block(x, w)
+        s.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("T", [9, 1500])
+def test_captured_and_replayed(T):
+    x, w, wd = _rand(T, 256, spread=0.5), _rand(2048, 256, seed=1, spread=0.3) * 0.06, _rand(256, 1024, seed=2, spread=0.3) * 0.03
+    kept = [fb.quantize_fp8_block(t, tile=True)[0] for t in (w, wd)]
+    new = _rand(T, 256, seed=5, spread=0.5)
+    with torch.no_grad():
+        want = [fb.gated_mlp_fp8_block(v, kept[0], None, kept[1]) for v in (x, new)]
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            fb.gated_mlp_fp8_block(x, kept[0], None, kept[1])
+        torch.cuda.current_stream().wait_stream(s)
+        g = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()]
+        out = []
+        for graph in g:
+            with torch.cuda.graph(graph):
+                out.append(fb.gated_mlp_fp8_block(x, kept[0], None, kept[1]))
+        for graph, o in zip(g, out):
+            graph.replay()
+            assert torch.equal(o, want[0])
+        x.copy_(new)
+        for graph in g:
+            graph.replay()
+        assert torch.equal(out[0], want[1]) and torch.equal(out[1], want[1])
+
+
+def test_training_step_captured_and_replayed():
+    x, w, dy = _rand(300, 256, spread=0.5), _rand(512, 256, seed=1, spread=0.3), _rand(300, 512, seed=2, spread=1.0)
+    x.requires_grad_(), w.requires_grad_()
+    step = lambda: torch.autograd.grad(fb.linear_fp8_block(x, w), (x, w), dy)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        want = [t.clone() for t in step()]
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    nv.check_status()
+
+
+def test_rows_behind_the_last_do_not_matter():
+    """A batch padded to a longer one: its own rows are what they are without the padding."""
+    x, w = _rand(200, 512, spread=1.0), _rand(256, 512, seed=1, spread=0.5)
+    q, _ = fb.quantize_fp8_block(w, tile=True)
+    wide = torch.full((333, 512), float("nan"), device="cuda", dtype=torch.bfloat16)
+    wide[:200] = x
+    with torch.no_grad():
+        assert torch.equal(fb.linear_fp8_block(wide, q)[:200], fb.linear_fp8_block(x, q))
+
+
+# ------------------------------------------------------------------------------------------------
+# Models
+# ------------------------------------------------------------------------------------------------
+def test_a_run_through_models_training_and_encoding():
+    """The recipe in the engine, its gradients beside the bf16 ones, and the trained kind of model encoding with kept
+    weights."""
+    from lset_b200.models import Qwen3Config
+    from lset_b200.train.data.collator import PackedCollator
+    from lset_b200.train.data.dataset import SyntheticPairDataset
+    from lset_b200.train.engine import TrainingEngine
+    from lset_b200.train.quantization.fp8 import Float8Linear, Fp8KeptLinear, apply_fp8_inference
+
+    cfg = Qwen3Config(vocab_size=2048, hidden_size=256, intermediate_size=512, num_hidden_layers=2,
+                      num_attention_heads=4, num_key_value_heads=2, head_dim=128)
+    ds = SyntheticPairDataset(64, 2048, (8, 24), (40, 200), seed=3)
+    batch = PackedCollator()([ds[i] for i in range(8)])
+
+    def engine(fused, **kw):
+        torch.manual_seed(0)
+        return TrainingEngine("qwen3", None, None, batch_size=8, lr=1e-3, packed=True, model_config=cfg,
+                              log_interval=0, scheduler_type="constant", fused_projections=fused, device="cuda", **kw)
+
+    for fused in (True, False):
+        ref, eng = engine(fused), engine(fused, fp8=True, fp8_recipe="block128")
+        assert sum(isinstance(m, Float8Linear) for m in eng.model.modules()) == (8 if fused else 14)
+        l_ref, l_fp8 = float(ref.forward_backward(batch, True)), float(eng.forward_backward(batch, True))
+        nv.check_status()
+        assert abs(l_fp8 - l_ref) < 0.1 * max(1.0, abs(l_ref))
+        flat = lambda e: torch.cat([g.flat_grad.float().cpu() for g in e.store.groups])  # noqa: E731
+        # an e4m3 value is off by 2^-4 / sqrt(3) of itself in the mean: a few percent a product, over two layers
+        assert torch.nn.functional.cosine_similarity(flat(eng), flat(ref), dim=0).item() > 0.95
+        eng.optimizer_step()
+
+    model = ref.model.eval()
+    ids = torch.randint(0, 2048, (3, 50), device="cuda")
+    with torch.no_grad():
+        want = model(ids)["hidden_states"].float()
+        apply_fp8_inference(model)
+        got = model(ids)["hidden_states"].float()
+    assert sum(isinstance(m, Fp8KeptLinear) for m in model.modules()) == 2 * 6
+    assert torch.nn.functional.cosine_similarity(got, want, dim=-1).min().item() > 0.97
+    nv.check_status()
