@@ -9,17 +9,15 @@
 #include <stdint.h>
 
 #include "../common/pdl.h"
-#include "../row/glu.cuh"
+#include "../common/row.cuh"
 #include "block_gemm.h"
+#include "block_glu.cuh"
 #include "block_scale.cuh"
 
 namespace lb {
 namespace {
 
 using bf16 = __nv_bfloat16;
-
-__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 // The bytes of four words of a 4 x 4 block, transposed.
 __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
@@ -54,161 +52,177 @@ __device__ __forceinline__ void store_scale(const BlockOut& o, long long r, int 
 constexpr int kTile = 128;
 struct CastSmem {
   uint32_t tile[kTile * kTile / 4];  // [column][four rows]
-  uint32_t part[8][64];              // a warp's maxima of its 128 columns, two a word
+  uint32_t part[16][64];             // a warp's maxima of its 128 columns, two a word
   uint32_t all[8];
 };
 
-// The 128 x 128 tile at (r0, c0) of a matrix [R, C] that the CTA's 256 threads hold in registers: thread
-// (rg, cg) = (threadIdx.x / 16, % 16) has rows rg * 4 + 64 u + i, columns cg * 8 .. cg * 8 + 7 in v[u][i]
-// (zeros outside the matrix). TILED: one scale for the tile; else `out` has one for each row and `out_t`
-// for each column. Either may be absent (data null).
+enum { kRows = 1, kCols = 2 };
+
+// The 128 x 128 tile at (r0, c0) of a matrix [R, C] that the CTA's 512 / U threads hold in registers: thread
+// (rq, cg) = (threadIdx.x / 16, % 16) has rows rq * 4 + 64 u + i, columns cg * 8 .. cg * 8 + 7 in v[u][i]
+// (zeros outside the matrix). WANT kRows: to `out`, kCols: transposed to `out_t`. TILED: one scale for the
+// tile; else `out` has one for each row and `out_t` for each column.
 //
 // Magnitudes are compared as integers (bf16 bits without the sign), two at a time, which also lets NaN and
-// infinities through to the top.
-template <int TILED, int E5M2>
-__device__ __forceinline__ void cast_tile(const uint4 (&v)[2][4], CastSmem& sm, int r0, int c0, int R, int C,
+// infinities through to the top. Bound by issued instructions before memory (4 bytes a value, read and both
+// outputs), so a value is unpacked once for both, scaled two at a time, and a lane stores one scale.
+template <int TILED, int E5M2, int WANT, int U>
+__device__ __forceinline__ void cast_tile(const uint4 (&v)[U][4], CastSmem& sm, int r0, int c0, int R, int C,
                                           const BlockOut& out, const BlockOut& out_t) {
+  constexpr int kWarps = 16 / U, kMine = 4 * U, kPairs = kMine / 2;   // rows of a thread; row p with p + kPairs a word
   const int cg = threadIdx.x & 15, rq = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = c0 + cg * 8;
   constexpr uint32_t kAbs = 0x7fff7fffu;
   uint32_t col[4] = {0u, 0u, 0u, 0u};   // maxima of the thread's eight columns
-  uint32_t row[4];                      // of its eight rows: rows i (low half) and i + 64
+  uint32_t row[kPairs];                 // and of its rows
+  {
+    uint32_t m[kMine];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t m[2];
+    for (int p = 0; p < kMine; ++p) {
+      const uint4& q = v[p / 4][p % 4];
+      const uint32_t w[4] = {q.x & kAbs, q.y & kAbs, q.z & kAbs, q.w & kAbs};
+      if (TILED || (WANT & kCols)) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t w[4] = {v[u][i].x & kAbs, v[u][i].y & kAbs, v[u][i].z & kAbs, v[u][i].w & kAbs};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) col[j] = __vmaxu2(col[j], w[j]);
-      m[u] = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
-      m[u] = __vmaxu2(m[u], m[u] >> 16);
+        for (int j = 0; j < 4; ++j) col[j] = __vmaxu2(col[j], w[j]);
+      }
+      if (!TILED && (WANT & kRows)) m[p] = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
     }
-    row[i] = __byte_perm(m[0], m[1], 0x5410);
+    if (!TILED && (WANT & kRows)) {
+#pragma unroll
+      for (int p = 0; p < kPairs; ++p)
+        row[p] = __vmaxu2(__byte_perm(m[p], m[p + kPairs], 0x5410), __byte_perm(m[p], m[p + kPairs], 0x7632));
+    }
   }
-  uint32_t tile_max = 0u;
+  float rs[kMine];
+  f2 cs[4];
   if (TILED) {
     uint32_t m = __vmaxu2(__vmaxu2(col[0], col[1]), __vmaxu2(col[2], col[3]));
-    m = max(m & 0xffffu, m >> 16);
-    m = __reduce_max_sync(0xffffffffu, m);
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
     if (lane == 0) sm.all[warp] = m;
     __syncthreads();
+    m = 0u;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) tile_max = max(tile_max, sm.all[k]);
+    for (int k = 0; k < kWarps; ++k) m = max(m, sm.all[k]);
+    const float s = block_inverse<E5M2>(m);
+    const uint32_t e = block_scale_byte<E5M2>(m);
+    cs[0] = cs[1] = cs[2] = cs[3] = f2_of(s, s);
+    if (threadIdx.x < kTile) {
+      if ((WANT & kRows) && r0 + threadIdx.x < R) store_scale(out, r0 + threadIdx.x, c0 / kTile, c0 + kTile >= C, e);
+      if ((WANT & kCols) && c0 + threadIdx.x < C) store_scale(out_t, c0 + threadIdx.x, r0 / kTile, r0 + kTile >= R, e);
+    }
   } else {
-    if (out.data != nullptr)
+    if (WANT & kRows) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int p = 0; p < kPairs; ++p) {
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) row[i] = __vmaxu2(row[i], __shfl_xor_sync(0xffffffffu, row[i], o));
-    if (out_t.data != nullptr) {
+        for (int o = 8; o > 0; o >>= 1) row[p] = __vmaxu2(row[p], __shfl_xor_sync(0xffffffffu, row[p], o));
+        rs[p] = block_inverse<E5M2>(row[p] & 0xffffu);
+        rs[p + kPairs] = block_inverse<E5M2>(row[p] >> 16);
+      }
+      if (cg < kMine) {   // lane cg stores the scale of row cg of the thread's
+        uint32_t w = row[0];
+#pragma unroll
+        for (int p = 1; p < kPairs; ++p) w = cg % kPairs == p ? row[p] : w;
+        const int r = r0 + rq * 4 + (cg & 3) + (cg >> 2) * 64;
+        if (r < R)
+          store_scale(out, r, c0 / kTile, c0 + kTile >= C, block_scale_byte<E5M2>(cg >= kPairs ? w >> 16 : w & 0xffffu));
+      }
+    }
+    if (WANT & kCols) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) col[j] = __vmaxu2(col[j], __shfl_xor_sync(0xffffffffu, col[j], 16));
       if (lane < 16)
         *reinterpret_cast<uint4*>(&sm.part[warp][cg * 4]) = make_uint4(col[0], col[1], col[2], col[3]);
       __syncthreads();
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < kWarps; ++k) {
         const uint4 p = *reinterpret_cast<const uint4*>(&sm.part[k][cg * 4]);
         col[0] = __vmaxu2(col[0], p.x);
         col[1] = __vmaxu2(col[1], p.y);
         col[2] = __vmaxu2(col[2], p.z);
         col[3] = __vmaxu2(col[3], p.w);
       }
-    }
-  }
-  const uint32_t tile_e = block_scale_byte<E5M2>(tile_max);
-  const float tile_inv = block_inverse(tile_e);
-  const bool tile_ok = block_is_finite(tile_max);
-
-  if (out.data != nullptr) {
-    const int kb = c0 / kTile;
-    const bool last = c0 + kTile >= C;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = r0 + rq * 4 + u * 64 + i;
-        const uint32_t top = TILED ? tile_max : (row[i] >> (16 * u)) & 0xffffu;
-        const uint32_t e = TILED ? tile_e : block_scale_byte<E5M2>(top);
-        const bool ok = TILED ? tile_ok : block_is_finite(top);
-        const float s = TILED ? tile_inv : block_inverse(e);
-        if (r < R) {
-          if (c < C) {
-            const uint4& q = v[u][i];
-            uint2 b = make_uint2(cast4<E5M2>(bf16_lo(q.x) * s, bf16_hi(q.x) * s, bf16_lo(q.y) * s, bf16_hi(q.y) * s),
-                                 cast4<E5M2>(bf16_lo(q.z) * s, bf16_hi(q.z) * s, bf16_lo(q.w) * s, bf16_hi(q.w) * s));
-            if (!ok) b = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
-            *reinterpret_cast<uint2*>(out.data + (long long)r * out.ld + c) = b;
-          }
-          if (cg == 0) store_scale(out, r, kb, last, ok ? e : kScaleOne);
-        }
-      }
-  }
-  if (out_t.data == nullptr) return;
-  uint32_t ce[8];
-  float cs[8];
-  bool cok[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t top = TILED ? tile_max : (col[j / 2] >> (16 * (j & 1))) & 0xffffu;
-    ce[j] = TILED ? tile_e : block_scale_byte<E5M2>(top);
-    cs[j] = TILED ? tile_inv : block_inverse(ce[j]);
-    cok[j] = TILED ? tile_ok : block_is_finite(top);
-  }
-  if (rq == 0 && c < C) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      store_scale(out_t, c + j, r0 / kTile, r0 + kTile >= R, cok[j] ? ce[j] : kScaleOne);
-  }
-  // Word `rg` (four rows) of a column of group cg lies at rg ^ 2 cg: the words that a warp writes at a time
-  // are in different banks, and four of a column stay together for the 16-byte reads.
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int rg = rq + u * 16;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      uint32_t q[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t a = k ? v[u][i].z : v[u][i].x, b = k ? v[u][i].w : v[u][i].y;
-        q[i] = cast4<E5M2>(bf16_lo(a) * cs[4 * k], bf16_hi(a) * cs[4 * k + 1], bf16_lo(b) * cs[4 * k + 2],
-                          bf16_hi(b) * cs[4 * k + 3]);
-      }
-      transpose4(q);
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        sm.tile[(cg * 8 + k * 4 + j) * 32 + (rg ^ (2 * cg))] = cok[4 * k + j] ? q[j] : 0x7f7f7f7fu;
+        cs[j] = f2_of(block_inverse<E5M2>(col[j] & 0xffffu), block_inverse<E5M2>(col[j] >> 16));
+      if (rq < 8 && c < C) {   // thread row rq stores the scale of column rq of the thread's eight
+        const uint32_t w = rq & 4 ? (rq & 2 ? col[3] : col[2]) : (rq & 2 ? col[1] : col[0]);
+        store_scale(out_t, c + rq, r0 / kTile, r0 + kTile >= R, block_scale_byte<E5M2>(rq & 1 ? w >> 16 : w & 0xffffu));
+      }
     }
   }
-  __syncthreads();
-  // row c of out_t holds column c of the tile: 16 rows of it a piece
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int tc = (threadIdx.x >> 3) + k * 32, m = threadIdx.x & 7, g = tc >> 3;
-    uint4 w = *reinterpret_cast<const uint4*>(sm.tile + tc * 32 + 4 * (m ^ (g >> 1)));
-    if (g & 1) w = make_uint4(w.z, w.w, w.x, w.y);
-    if (c0 + tc < C && r0 + m * 16 < out_t.ld)
-      *reinterpret_cast<uint4*>(out_t.data + (long long)(c0 + tc) * out_t.ld + r0 + m * 16) = w;
-  }
-}
 
-__device__ __forceinline__ void load_tile(uint4 (&v)[2][4], const bf16* __restrict__ x, long long ldx, int r0,
-                                          int c0, int R, int C) {
-  const int c = c0 + (threadIdx.x & 15) * 8;
+  // Word `rg` (four rows) of a column of group cg lies at rg ^ 2 cg: the words that a warp writes at a time
+  // are in different banks, and four of a column stay together for the 16-byte reads.
+  uint8_t* orow = WANT & kRows ? out.data + (long long)(r0 + rq * 4) * out.ld + c : nullptr;
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
+  for (int u = 0; u < U; ++u) {
+    uint32_t b[4][2];
+    uint32_t q[2][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = r0 + (threadIdx.x >> 4) * 4 + u * 64 + i;
-      v[u][i] = r < R && c < C ? *reinterpret_cast<const uint4*>(x + r * ldx + c) : make_uint4(0u, 0u, 0u, 0u);
+      const uint32_t w[4] = {v[u][i].x, v[u][i].y, v[u][i].z, v[u][i].w};
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const f2 lo = f2_bf16(w[2 * k]), hi = f2_bf16(w[2 * k + 1]);
+        if (TILED || (WANT & kCols)) {
+          const float2 x = f2_get(f2_mul(lo, cs[2 * k])), y = f2_get(f2_mul(hi, cs[2 * k + 1]));
+          q[k][i] = cast4<E5M2>(x.x, x.y, y.x, y.y);
+        }
+        if (TILED) {
+          b[i][k] = q[k][i];
+        } else if (WANT & kRows) {
+          const f2 s = f2_of(rs[4 * u + i], rs[4 * u + i]);
+          const float2 x = f2_get(f2_mul(lo, s)), y = f2_get(f2_mul(hi, s));
+          b[i][k] = cast4<E5M2>(x.x, x.y, y.x, y.y);
+        }
+      }
+      if (WANT & kRows) {
+        if (r0 + rq * 4 + u * 64 + i < R && c < C)
+          *reinterpret_cast<uint2*>(orow + (u * 64 + i) * out.ld) = make_uint2(b[i][0], b[i][1]);
+      }
     }
+    if (WANT & kCols) {
+      const int rg = rq + u * 16;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        transpose4(q[k]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sm.tile[(cg * 8 + k * 4 + j) * 32 + (rg ^ (2 * cg))] = q[k][j];
+      }
+    }
+  }
+  if (!(WANT & kCols)) return;
+  __syncthreads();
+  // row c of out_t holds column c of the tile: 16 rows of it a piece
+  const int m = threadIdx.x & 7, tc0 = threadIdx.x >> 3;
+  uint8_t* ocol = out_t.data + (long long)(c0 + tc0) * out_t.ld + r0 + m * 16;
+#pragma unroll
+  for (int k = 0; k < 2 * U; ++k) {
+    const int tc = tc0 + k * (64 / U), g = tc >> 3;
+    uint4 w = *reinterpret_cast<const uint4*>(sm.tile + tc * 32 + 4 * (m ^ (g >> 1)));
+    if (g & 1) w = make_uint4(w.z, w.w, w.x, w.y);
+    if (c0 + tc < C && r0 + m * 16 < out_t.ld) *reinterpret_cast<uint4*>(ocol + k * (64 / U) * out_t.ld) = w;
+  }
 }
 
-// colsum (where it is wanted: the gradient of a bias): the tile's column sums to row r0 / 128 of a matrix
-// [.., C], always added in the same order.
-template <int TILED, int E5M2>
-__global__ void __launch_bounds__(256)
+template <int U>
+__device__ __forceinline__ void load_tile(uint4 (&v)[U][4], const bf16* __restrict__ x, long long ldx, int r0,
+                                          int c0, int R, int C) {
+  const int c = c0 + (threadIdx.x & 15) * 8, r = r0 + (threadIdx.x >> 4) * 4;
+  const bf16* p = x + r * ldx + c;
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[u][i] = r + u * 64 + i < R && c < C ? *reinterpret_cast<const uint4*>(p + (u * 64 + i) * ldx)
+                                            : make_uint4(0u, 0u, 0u, 0u);
+}
+
+// SUM (the gradient of a bias): the tile's column sums too, to row r0 / 128 of `colsum` [.., C], always added
+// in the same order.
+template <int TILED, int E5M2, int WANT, int SUM>
+__global__ void __launch_bounds__(256, 4)
     block_cast_kernel(const bf16* __restrict__ x, int R, int C, long long ldx, BlockOut out, BlockOut out_t,
                       float* __restrict__ colsum, int tiles_c) {
   __shared__ __align__(16) CastSmem sm;
@@ -218,41 +232,44 @@ __global__ void __launch_bounds__(256)
   const int r0 = rt * kTile, c0 = (blockIdx.x - rt * tiles_c) * kTile;
   uint4 v[2][4];
   load_tile(v, x, ldx, r0, c0, R, C);
-  if (!TILED && colsum != nullptr) {
-    float s[8];
+  if (SUM) {
+    f2 s[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      s[j] = 0.f;
+    for (int j = 0; j < 4; ++j) s[j] = f2_of(0.f, 0.f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint4& q = v[k / 4][k % 4];
-        const uint32_t w = j / 2 == 0 ? q.x : (j / 2 == 1 ? q.y : (j / 2 == 2 ? q.z : q.w));
-        s[j] += j & 1 ? bf16_hi(w) : bf16_lo(w);
-      }
-      s[j] += __shfl_xor_sync(0xffffffffu, s[j], 16);
+    for (int k = 0; k < 8; ++k) {
+      f2 t[4];
+      unpack8(v[k / 4][k % 4], t);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[j] = f2_add(s[j], t[j]);
     }
-    float* part = reinterpret_cast<float*>(sm.tile);   // [8 warps][128 columns]
-    const int warp = threadIdx.x >> 5, cg = threadIdx.x & 15;
-    if ((threadIdx.x & 31) < 16) {
+    float* part = reinterpret_cast<float*>(sm.tile);   // [16 thread rows][128 columns]
 #pragma unroll
-      for (int j = 0; j < 8; ++j) part[warp * kTile + cg * 8 + j] = s[j];
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = f2_get(s[j]);
+      *reinterpret_cast<float2*>(part + (threadIdx.x >> 4) * kTile + (threadIdx.x & 15) * 8 + 2 * j) = t;
     }
     __syncthreads();
     if (threadIdx.x < kTile && c0 + threadIdx.x < C) {
       float t = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) t += part[k * kTile + threadIdx.x];
+      for (int k = 0; k < 16; ++k) t += part[k * kTile + threadIdx.x];
       colsum[(long long)rt * C + c0 + threadIdx.x] = t;
     }
     __syncthreads();
+    // (the unpacked values are not to be kept for the cast: they would fill the registers of two CTAs)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      uint4& q = v[k / 4][k % 4];
+      asm volatile("" : "+r"(q.x), "+r"(q.y), "+r"(q.z), "+r"(q.w));
+    }
   }
-  cast_tile<TILED, E5M2>(v, sm, r0, c0, R, C, out, out_t);
+  if (WANT) cast_tile<TILED, E5M2, WANT, 2>(v, sm, r0, c0, R, C, out, out_t);
 }
 
-// h = act(gate) * up of [T, I] matrices (rows ld elements apart), rounded to bf16 as the separate activation
-// rounds it, in blocks of a row.
+// h = act(gate) * up of [T, I] matrices (rows ld elements apart), rounded to bf16, in blocks of a row.
 template <int KIND>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
     block_glu_fwd_kernel(const bf16* __restrict__ gate, const bf16* __restrict__ up, long long ld, int T, int I,
                          BlockOut h, int tiles_c) {
   __shared__ __align__(16) CastSmem sm;
@@ -260,22 +277,20 @@ __global__ void __launch_bounds__(256)
   pdl_trigger();
   const int rt = blockIdx.x / tiles_c;
   const int r0 = rt * kTile, c0 = (blockIdx.x - rt * tiles_c) * kTile;
-  uint4 g[2][4], u[2][4];
+  uint4 g[1][4], u[1][4];
   load_tile(g, gate, ld, r0, c0, T, I);
   load_tile(u, up, ld, r0, c0, T, I);
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) g[k][i] = glu_fwd8<KIND>(g[k][i], u[k][i]);
-  cast_tile<0, 0>(g, sm, r0, c0, T, I, h, BlockOut{});
+  for (int i = 0; i < 4; ++i) g[0][i] = block_glu8<KIND>(g[0][i], u[0][i]);
+  cast_tile<0, 0, kRows, 1>(g, sm, r0, c0, T, I, h, BlockOut{});
 }
 
 // The way back: from dh, gate and up the gradients of gate and up (rounded to bf16) in blocks of a row (`d`
 // [T, 2 I], gate columns first) and of 128 tokens (`d_t` [2 I, T]), and h once more, in blocks of 128 tokens
 // (`h_t` [I, T]): the operands of the input gradient and of both weight gradients from one read. I is a
-// multiple of 128, so that no block holds columns of both.
-template <int KIND>
-__global__ void __launch_bounds__(256, 2)
+// multiple of 128, so that no block holds columns of both. WANT: of the gradients' layouts; H: h.
+template <int KIND, int WANT, int H>
+__global__ void __launch_bounds__(512, 2)
     block_glu_bwd_kernel(const bf16* __restrict__ dh, long long ld_dh, const bf16* __restrict__ gate,
                          const bf16* __restrict__ up, long long ld, int T, int I, BlockOut d, BlockOut d_t,
                          BlockOut h_t, int tiles_c) {
@@ -284,24 +299,21 @@ __global__ void __launch_bounds__(256, 2)
   pdl_trigger();
   const int rt = blockIdx.x / tiles_c;
   const int r0 = rt * kTile, c0 = (blockIdx.x - rt * tiles_c) * kTile;
-  uint4 g[2][4], u[2][4], x[2][4];
+  uint4 g[1][4], u[1][4], x[1][4];
   load_tile(g, gate, ld, r0, c0, T, I);
   load_tile(u, up, ld, r0, c0, T, I);
   load_tile(x, dh, ld_dh, r0, c0, T, I);
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 h = glu_fwd8<KIND>(g[k][i], u[k][i]);
-      glu_bwd8<KIND>(g[k][i], u[k][i], x[k][i], g[k][i], u[k][i]);
-      x[k][i] = h;
-    }
-  cast_tile<0, 0>(g, sm, r0, c0, T, 2 * I, d, d_t);
-  __syncthreads();
-  cast_tile<0, 0>(u, sm, r0, I + c0, T, 2 * I, d, d_t);
-  if (h_t.data == nullptr) return;
-  __syncthreads();
-  cast_tile<0, 0>(x, sm, r0, c0, T, I, BlockOut{}, h_t);
+  for (int i = 0; i < 4; ++i) block_glu_grad8<KIND>(g[0][i], u[0][i], x[0][i]);
+  if (WANT) {
+    cast_tile<0, 0, WANT, 1>(g, sm, r0, c0, T, 2 * I, d, d_t);
+    __syncthreads();
+    cast_tile<0, 0, WANT, 1>(u, sm, r0, I + c0, T, 2 * I, d, d_t);
+  }
+  if (H) {
+    __syncthreads();
+    cast_tile<0, 0, kCols, 1>(x, sm, r0, c0, T, I, BlockOut{}, h_t);
+  }
 }
 
 // out [rows, cols] = (out +) sums of P matrices, part p at p * stride, each value in the order of p.
@@ -355,11 +367,33 @@ int block_cast(const void* x, int R, int C, long long ldx, int tiled, int e5m2, 
   if (R <= 0 || C <= 0) return 0;
   if ((C & 7) || (ldx & 7) || (reinterpret_cast<uintptr_t>(x) & 15)) return -3;
   if (!fits(out, R, C) || !fits(out_t, C, R) || kb0_t < 0 || (kb0_t > 0 && (R % kTile))) return -3;
-  if (colsum != nullptr && tiled) return -5;
   const unsigned grid = cast_grid(R, C);
   if (grid == 0) return -3;
-  auto kern = tiled ? (e5m2 ? block_cast_kernel<1, 1> : block_cast_kernel<1, 0>)
-                    : (e5m2 ? block_cast_kernel<0, 1> : block_cast_kernel<0, 0>);
+  const int want = (out.data != nullptr ? kRows : 0) | (out_t.data != nullptr ? kCols : 0);
+  if (want == 0 && colsum == nullptr) return 0;
+#define LB_CAST(TI, E, W, S) \
+  if (tiled == TI && e5m2 == E && want == W && (colsum != nullptr) == S) kern = block_cast_kernel<TI, E, W, S>
+  void (*kern)(const bf16*, int, int, long long, BlockOut, BlockOut, float*, int) = nullptr;
+  tiled = tiled ? 1 : 0;
+  e5m2 = e5m2 ? 1 : 0;
+  LB_CAST(0, 0, 1, 0);
+  LB_CAST(0, 0, 2, 0);
+  LB_CAST(0, 0, 3, 0);
+  LB_CAST(0, 1, 1, 0);
+  LB_CAST(0, 1, 2, 0);
+  LB_CAST(0, 1, 3, 0);
+  LB_CAST(1, 0, 1, 0);
+  LB_CAST(1, 0, 2, 0);
+  LB_CAST(1, 0, 3, 0);
+  LB_CAST(1, 1, 1, 0);
+  LB_CAST(1, 1, 2, 0);
+  LB_CAST(1, 1, 3, 0);
+  LB_CAST(0, 0, 0, 1);
+  LB_CAST(0, 0, 1, 1);
+  LB_CAST(0, 0, 2, 1);
+  LB_CAST(0, 0, 3, 1);
+#undef LB_CAST
+  if (kern == nullptr) return -5;
   return launch_pdl(kern, dim3(grid), dim3(256), 0, stream, pdl_enabled(4LL * R * C), 1,
                     static_cast<const bf16*>(x), R, C, ldx, block_out(out), block_out(out_t, kb0_t), colsum,
                     (C + kTile - 1) / kTile);
@@ -374,7 +408,7 @@ int block_glu_fwd(int kind, const void* gate, const void* up, long long ld, int 
   const unsigned grid = cast_grid(T, I);
   if (grid == 0) return -3;
   return launch_pdl(kind == kSwiglu ? block_glu_fwd_kernel<kSwiglu> : block_glu_fwd_kernel<kGeglu>, dim3(grid),
-                    dim3(256), 0, stream, pdl_enabled(5LL * T * I), 1, static_cast<const bf16*>(gate),
+                    dim3(512), 0, stream, pdl_enabled(5LL * T * I), 1, static_cast<const bf16*>(gate),
                     static_cast<const bf16*>(up), ld, T, I, block_out(out), I / kTile);
 }
 
@@ -387,8 +421,21 @@ int block_glu_bwd(int kind, const void* dh, long long ld_dh, const void* gate, c
   if (!fits(d, T, 2LL * I) || !fits(d_t, 2LL * I, T) || !fits(h_t, I, T)) return -3;
   const unsigned grid = cast_grid(T, I);
   if (grid == 0) return -3;
-  return launch_pdl(kind == kSwiglu ? block_glu_bwd_kernel<kSwiglu> : block_glu_bwd_kernel<kGeglu>, dim3(grid),
-                    dim3(256), 0, stream, pdl_enabled(11LL * T * I), 1, static_cast<const bf16*>(dh), ld_dh,
+  const int want = (d.data != nullptr ? kRows : 0) | (d_t.data != nullptr ? kCols : 0), h = h_t.data != nullptr;
+  if (want == 0 && h == 0) return 0;
+#define LB_GLU(W, H) \
+  if (want == W && h == H) kern = kind == kSwiglu ? block_glu_bwd_kernel<kSwiglu, W, H> : block_glu_bwd_kernel<kGeglu, W, H>
+  void (*kern)(const bf16*, long long, const bf16*, const bf16*, long long, int, int, BlockOut, BlockOut, BlockOut,
+               int) = nullptr;
+  LB_GLU(0, 1);
+  LB_GLU(1, 0);
+  LB_GLU(1, 1);
+  LB_GLU(2, 0);
+  LB_GLU(2, 1);
+  LB_GLU(3, 0);
+  LB_GLU(3, 1);
+#undef LB_GLU
+  return launch_pdl(kern, dim3(grid), dim3(512), 0, stream, pdl_enabled(11LL * T * I), 1, static_cast<const bf16*>(dh), ld_dh,
                     static_cast<const bf16*>(gate), static_cast<const bf16*>(up), ld, T, I, block_out(d),
                     block_out(d_t), block_out(h_t), I / kTile);
 }

@@ -23,8 +23,12 @@ struct BlockMat {
 // second launch adds up.
 struct BlockPlan {
   int kernel, tn, splits;
+  float cost;   // modelled, us
 };
-BlockPlan block_plan(int M, int N, int K, int out_fp32, int accumulate, bool bias, bool aligned);
+// aligned: C may be written in pieces of 16 bytes, which the pair kernel does.
+BlockPlan block_plan(int M, int N, int K, bool aligned);
+// Whether block_gemm_glu is the faster way to the gated projections of T rows.
+bool block_glu_fused(int T, int I, int K);
 // Bytes of temporary storage of a plan.
 size_t block_plan_bytes(const BlockPlan& p, int M, int N);
 
@@ -41,7 +45,6 @@ int block_gemm_2cta(int splits, long long split_stride, const BlockMat& A, const
                     cudaStream_t stream);
 // Whether `splits` divides the contraction into that many parts (whole groups of scale words each).
 bool block_2cta_splits_ok(int K, int splits);
-int block_2cta_pairs();
 // h = act(A · Wgᵀ) * (A · Wuᵀ), cast; Wu's rows follow Wg's scale words in one group. See gemm_block_2cta.cu.
 int block_gemm_glu(int kind, const BlockMat& A, const BlockMat& Wg, const BlockMat& Wu, int M, int I, int K,
                    void* gate, void* up, long long ld_gu, const BlockMat& h, int* status, cudaStream_t stream);

@@ -63,17 +63,14 @@ struct Call {
   void product(const BlockMat& a, const BlockMat& b, const Out& out, int M, int N, int K, long long ldc,
                const void* bias = nullptr) {
     run([&] {
-      const BlockPlan p = block_plan(M, N, K, out.mode > 0, out.mode == 2, bias != nullptr,
-                                     aligned16(out.p) && !(N & 7) && !(ldc & 7));
+      const BlockPlan p = block_plan(M, N, K, aligned16(out.p) && !(N & 7) && !(ldc & 7));
       return block_gemm(p, a, b, out.p, M, N, K, ldc, out.mode > 0, out.mode == 2, bias, ws, status, stream);
     });
   }
 };
 
 // Storage of a product whatever the alignment of its output.
-size_t product_bytes(int M, int N, int K, int mode) {
-  return block_plan_bytes(block_plan(M, N, K, mode > 0, mode == 2, false, !(N & 7)), M, N);
-}
+size_t product_bytes(int M, int N, int K) { return block_plan_bytes(block_plan(M, N, K, !(N & 7)), M, N); }
 size_t max2(size_t a, size_t b) { return a > b ? a : b; }
 
 struct LinearStorage {
@@ -83,7 +80,7 @@ struct LinearStorage {
   size_t saved, fwd, bwd;
 };
 
-LinearStorage linear_storage(int T, int K, int N, int need, int y_mode, int dw_mode, void* saved, void* tmp) {
+LinearStorage linear_storage(int T, int K, int N, int need, void* saved, void* tmp) {
   LinearStorage s{};
   const bool need_x = need & 1, need_w = need & 2, need_b = need & 4;
   Arena keep(saved), fwd(tmp), bwd(tmp);
@@ -91,11 +88,11 @@ LinearStorage linear_storage(int T, int K, int N, int need, int y_mode, int dw_m
   if (need_x) s.w_t = keep.mat(K, N);
   s.x = fwd.mat(T, K);
   s.w = fwd.mat(N, K);
-  s.ws_fwd = fwd.take(product_bytes(T, N, K, y_mode));
+  s.ws_fwd = fwd.take(product_bytes(T, N, K));
   if (need_x) s.dy = bwd.mat(T, N);
   if (need_w) s.dy_t = bwd.mat(N, T);
   if (need_b) s.colsum = static_cast<float*>(bwd.take(size_t((T + 127) / 128) * N * 4));
-  s.ws_bwd = bwd.take(max2(need_x ? product_bytes(T, K, N, y_mode) : 0, need_w ? product_bytes(N, K, T, dw_mode) : 0));
+  s.ws_bwd = bwd.take(max2(need_x ? product_bytes(T, K, N) : 0, need_w ? product_bytes(N, K, T) : 0));
   s.saved = keep.at;
   s.fwd = fwd.at;
   s.bwd = bwd.at;
@@ -110,7 +107,7 @@ struct MlpStorage {
 };
 
 // need: 1 = x, 2 = gate or up weight, 4 = down weight
-MlpStorage mlp_storage(int T, int H, int I, int need, const int* modes, void* saved, void* tmp) {
+MlpStorage mlp_storage(int T, int H, int I, int need, void* saved, void* tmp) {
   MlpStorage s{};
   const bool need_x = need & 1, need_gu = need & 2, need_d = need & 4;
   Arena keep(saved), fwd(tmp), bwd(tmp);
@@ -122,7 +119,7 @@ MlpStorage mlp_storage(int T, int H, int I, int need, const int* modes, void* sa
   s.w = fwd.mat(2LL * I, H);
   s.wd = fwd.mat(H, I);
   s.h = fwd.mat(T, I);
-  s.ws_fwd = fwd.take(max2(product_bytes(T, 2 * I, H, 0), product_bytes(T, H, I, 0)));
+  s.ws_fwd = fwd.take(max2(product_bytes(T, 2 * I, H), product_bytes(T, H, I)));
   if (need_x || need_gu) {
     s.dy = bwd.mat(T, H);
     s.dh = static_cast<__nv_bfloat16*>(bwd.take(size_t(T) * I * 2));
@@ -132,11 +129,10 @@ MlpStorage mlp_storage(int T, int H, int I, int need, const int* modes, void* sa
   if (need_gu) s.d_t = bwd.mat(2LL * I, T);
   if (need_d) s.h_t = bwd.mat(I, T);
   size_t ws = 0;
-  if (need_x || need_gu) ws = max2(ws, product_bytes(T, I, H, 0));
-  if (need_x) ws = max2(ws, product_bytes(T, H, 2 * I, 0));
-  if (need_gu) ws = max2(ws, max2(product_bytes(2 * I, H, T, modes[0]), product_bytes(I, H, T, modes[0])));
-  if (need_gu) ws = max2(ws, product_bytes(I, H, T, modes[1]));
-  if (need_d) ws = max2(ws, product_bytes(H, I, T, modes[2]));
+  if (need_x || need_gu) ws = max2(ws, product_bytes(T, I, H));
+  if (need_x) ws = max2(ws, product_bytes(T, H, 2 * I));
+  if (need_gu) ws = max2(ws, max2(product_bytes(2 * I, H, T), product_bytes(I, H, T)));
+  if (need_d) ws = max2(ws, product_bytes(H, I, T));
   s.ws_bwd = bwd.take(ws);
   s.saved = keep.at;
   s.fwd = fwd.at;
@@ -144,13 +140,10 @@ MlpStorage mlp_storage(int T, int H, int I, int need, const int* modes, void* sa
   return s;
 }
 
-// The fused projection and activation on CTA pairs, or the products and a launch for the activation.
-bool fused_glu(int T, int I) { return 1LL * ((T + 255) / 256) * (I / 128) >= 40; }
-
 // y = (act(x Wgᵀ) * (x Wuᵀ)) Wdᵀ from cast operands; keep_gu: the products stay in s.gu.
 void mlp_products(Call& c, int kind, const MlpStorage& s, int T, int H, int I, bool keep_gu, void* y) {
   const BlockMat up = rows_of(s.w, I);
-  if (fused_glu(T, I)) {
+  if (block_glu_fused(T, I, H)) {
     c.run([&] {
       return block_gemm_glu(kind, s.x, s.w, up, T, I, H, keep_gu ? s.gu : nullptr, keep_gu ? s.gu + I : nullptr,
                             2LL * I, s.h, c.status, c.stream);
@@ -169,8 +162,8 @@ using namespace lb;
 
 // Bytes that the calls below want: out = {saved, tmp of the forward, tmp of the backward}. need: gradients of 1 = x,
 // 2 = weight, 4 = bias. Modes of outputs throughout: 0 = bf16, 1 = fp32, 2 = added to fp32.
-extern "C" int lb_linear_block_bytes(int T, int K, int N, int need, int y_mode, int dw_mode, long long* out) {
-  const LinearStorage s = linear_storage(T, K, N, need, y_mode, dw_mode, nullptr, nullptr);
+extern "C" int lb_linear_block_bytes(int T, int K, int N, int need, long long* out) {
+  const LinearStorage s = linear_storage(T, K, N, need, nullptr, nullptr);
   out[0] = (long long)s.saved;
   out[1] = (long long)s.fwd;
   out[2] = (long long)s.bwd;
@@ -182,7 +175,7 @@ extern "C" int lb_linear_block_fwd(const void* x, long long ldx, const void* w, 
                                    int T, int K, int N, int need, int y_mode, void* y, void* saved, void* tmp,
                                    int* status, void* stream_) {
   if (T <= 0 || K <= 0 || N <= 0) return -3;
-  const LinearStorage s = linear_storage(T, K, N, need, y_mode, 0, saved, tmp);
+  const LinearStorage s = linear_storage(T, K, N, need, saved, tmp);
   Call c{status, reinterpret_cast<cudaStream_t>(stream_), s.ws_fwd};
   c.run([&] { return block_cast(x, T, K, ldx, 0, 0, s.x, s.x_t, 0, nullptr, c.stream); });
   c.run([&] { return block_cast(w, N, K, ldw, 1, 0, s.w, s.w_t, 0, nullptr, c.stream); });
@@ -191,10 +184,10 @@ extern "C" int lb_linear_block_fwd(const void* x, long long ldx, const void* w, 
 }
 
 // The same with a weight in 8 bits (bytes, rows ldw apart; scale words, rows_w a group). tmp: lb_linear_kept_bytes.
-extern "C" long long lb_linear_kept_bytes(int T, int K, int N, int y_mode) {
+extern "C" long long lb_linear_kept_bytes(int T, int K, int N) {
   Arena a(nullptr);
   a.mat(T, K);
-  a.take(product_bytes(T, N, K, y_mode));
+  a.take(product_bytes(T, N, K));
   return (long long)a.at;
 }
 extern "C" int lb_linear_kept_fwd(const void* x, long long ldx, const void* w, long long ldw, const void* scales,
@@ -215,7 +208,7 @@ extern "C" int lb_linear_block_bwd(const void* dy, long long lddy, int T, int K,
                                    void* tmp, void* dx, int dx_mode, void* dw, int dw_mode, void* db, int db_mode,
                                    int* status, void* stream_) {
   if (T <= 0 || K <= 0 || N <= 0) return -3;
-  const LinearStorage s = linear_storage(T, K, N, need, dx_mode, dw_mode, saved, tmp);
+  const LinearStorage s = linear_storage(T, K, N, need, saved, tmp);
   Call c{status, reinterpret_cast<cudaStream_t>(stream_), s.ws_bwd};
   c.run([&] { return block_cast(dy, T, N, lddy, 0, 0, s.dy, s.dy_t, 0, s.colsum, c.stream); });
   if (need & 1) c.product(s.dy, s.w_t, Out{dx, dx_mode}, T, K, N, K);
@@ -227,8 +220,8 @@ extern "C" int lb_linear_block_bwd(const void* dy, long long lddy, int T, int K,
 
 // The gated block. need: gradients of 1 = x, 2 = the gate or up weight, 4 = the down weight; modes: of the gate (or
 // fused), up and down weights' gradients.
-extern "C" int lb_mlp_block_bytes(int T, int H, int I, int need, const int* modes, long long* out) {
-  const MlpStorage s = mlp_storage(T, H, I, need, modes, nullptr, nullptr);
+extern "C" int lb_mlp_block_bytes(int T, int H, int I, int need, long long* out) {
+  const MlpStorage s = mlp_storage(T, H, I, need, nullptr, nullptr);
   out[0] = (long long)s.saved;
   out[1] = (long long)s.fwd;
   out[2] = (long long)s.bwd;
@@ -240,8 +233,7 @@ extern "C" int lb_mlp_block_fwd(int kind, const void* x, long long ldx, const vo
                                 long long ldu, const void* wd, long long ldd, int T, int H, int I, int need, void* y,
                                 void* saved, void* tmp, int* status, void* stream_) {
   if (T <= 0 || H <= 0 || I <= 0 || (I % kScaleBlock)) return -3;
-  const int modes[3] = {0, 0, 0};
-  const MlpStorage s = mlp_storage(T, H, I, need, modes, saved, tmp);
+  const MlpStorage s = mlp_storage(T, H, I, need, saved, tmp);
   Call c{status, reinterpret_cast<cudaStream_t>(stream_), s.ws_fwd};
   c.run([&] { return block_cast(x, T, H, ldx, 0, 0, s.x, s.x_t, 0, nullptr, c.stream); });
   if (wu == nullptr) {
@@ -264,8 +256,8 @@ MlpStorage mlp_kept_storage(int T, int H, int I, void* tmp) {
   Arena a(tmp);
   s.x = a.mat(T, H);
   s.h = a.mat(T, I);
-  if (!fused_glu(T, I)) s.gu = static_cast<__nv_bfloat16*>(a.take(size_t(T) * 2 * I * 2));
-  s.ws_fwd = a.take(max2(product_bytes(T, 2 * I, H, 0), product_bytes(T, H, I, 0)));
+  if (!block_glu_fused(T, I, H)) s.gu = static_cast<__nv_bfloat16*>(a.take(size_t(T) * 2 * I * 2));
+  s.ws_fwd = a.take(max2(product_bytes(T, 2 * I, H), product_bytes(T, H, I)));
   s.fwd = a.at;
   return s;
 }
@@ -293,7 +285,7 @@ extern "C" int lb_mlp_block_bwd(int kind, const void* dy, long long lddy, int T,
                                 void* saved, void* tmp, void* dx, void* dwg, void* dwu, void* dwd, const int* modes,
                                 int* status, void* stream_) {
   if (T <= 0 || H <= 0 || I <= 0 || (I % kScaleBlock)) return -3;
-  const MlpStorage s = mlp_storage(T, H, I, need, modes, saved, tmp);
+  const MlpStorage s = mlp_storage(T, H, I, need, saved, tmp);
   Call c{status, reinterpret_cast<cudaStream_t>(stream_), s.ws_bwd};
   c.run([&] { return block_cast(dy, T, H, lddy, 0, 0, s.dy, s.dy_t, 0, nullptr, c.stream); });
   const bool inner = need & 3;

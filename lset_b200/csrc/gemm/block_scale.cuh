@@ -19,8 +19,6 @@
 // four blocks, and no row count needs padding.
 #pragma once
 
-#include <cuda_fp8.h>
-
 #include "../common/ptx.cuh"
 
 namespace lb {
@@ -28,24 +26,32 @@ namespace lb {
 constexpr int kScaleBlock = 128;
 constexpr uint32_t kScaleOne = 127u;
 
-// Scale byte of a block whose largest magnitude has the bf16 bits `a` (finite).
+// What the values of a block are multiplied by before they are rounded, 2^(127 - e) as float bits, for a block
+// whose largest magnitude has the bf16 bits `a`; NaN where that is not finite (and then so is every product).
+// (a + 31) / 128 is its exponent, plus one where the mantissa is above 0.75 = 96 / 128.
+template <int E5M2>
+__device__ __forceinline__ float block_inverse(uint32_t a) {
+  const int x = min((E5M2 ? 269 : 262) - int((a + 31u) >> 7), 253);
+  return __uint_as_float(a >= 0x7f80u ? 0x7fffffffu : uint32_t(x) << 23);
+}
+// The scale byte that goes with it.
 template <int E5M2>
 __device__ __forceinline__ uint32_t block_scale_byte(uint32_t a) {
-  if (a == 0u) return kScaleOne;
-  const int e = int(a >> 7) - (E5M2 ? 15 : 8) + ((a & 0x7fu) > 0x60u ? 1 : 0);
-  return uint32_t(min(max(e, 1), 254));
+  const int x = min((E5M2 ? 269 : 262) - int((a + 31u) >> 7), 253);
+  return a == 0u || a >= 0x7f80u ? kScaleOne : uint32_t(254 - x);
 }
-__device__ __forceinline__ bool block_is_finite(uint32_t a) { return a < 0x7f80u; }
-// 2^(127 - e): what a value is multiplied by before it is rounded.
-__device__ __forceinline__ float block_inverse(uint32_t e) { return __uint_as_float((254u - e) << 23); }
 
-// Four values, scaled already, as bytes.
+// Four values, scaled already, as bytes, to nearest even.
 template <int E5M2>
 __device__ __forceinline__ uint32_t cast4(float a, float b, float c, float d) {
-  constexpr __nv_fp8_interpretation_t kind = E5M2 ? __NV_E5M2 : __NV_E4M3;
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, kind);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, kind);
-  return lo | (hi << 16);
+  uint32_t o;
+  if (E5M2)
+    asm("{\n.reg .b16 lo, hi;\ncvt.rn.satfinite.e5m2x2.f32 lo, %2, %1;\ncvt.rn.satfinite.e5m2x2.f32 hi, %4, %3;\n"
+        "mov.b32 %0, {lo, hi};\n}" : "=r"(o) : "f"(a), "f"(b), "f"(c), "f"(d));
+  else
+    asm("{\n.reg .b16 lo, hi;\ncvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\ncvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n"
+        "mov.b32 %0, {lo, hi};\n}" : "=r"(o) : "f"(a), "f"(b), "f"(c), "f"(d));
+  return o;
 }
 
 // D[tmem] (+)= (A[smem] * scales) * (B[smem] * scales), 8-bit floats, 32 elements of depth. The scale

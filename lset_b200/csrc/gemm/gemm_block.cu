@@ -12,6 +12,7 @@
 //   warps 2-5   copy scale words from memory to TMEM ahead of the issuer (the instruction reads them from
 //               every quarter of the lanes: each warp writes its own), then drain the accumulator
 #include <cuda_bf16.h>
+#include <math.h>
 
 #include "../common/pdl.h"
 #include "../common/ptx.cuh"
@@ -48,6 +49,7 @@ struct BlockArgs {
   int a_e5m2, b_e5m2;
   int q_rows;                    // rows of A in a box: TN, or M where that is less
   int tiles_m;
+  int vec;                       // rows of C start at multiples of eight elements and 16 bytes
   int* status;
 };
 
@@ -66,20 +68,53 @@ __device__ __forceinline__ uint32_t cluster_size() {
   asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr, uint32_t rank) {
   uint32_t at;
-  float v;
+  float4 v;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
   return v;
 }
 
-__device__ __forceinline__ void store_c(const BlockArgs& g, int m, int n, float v, float bias) {
+// Eight columns from n on of row m of C, v their sums.
+__device__ __forceinline__ void store_c8(const BlockArgs& g, int m, int n, float (&v)[8]) {
+  if (g.bias != nullptr) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (n + i < g.N) v[i] += __bfloat162float(g.bias[n + i]);
+  }
+  const long long at = m * g.ldc + n;
+  const bool whole = g.vec && n + 8 <= g.N;
   if (g.out_fp32) {
-    float* p = static_cast<float*>(g.C) + m * g.ldc + n;
-    *p = v + (g.accumulate ? *p : bias);
+    float* p = static_cast<float*>(g.C) + at;
+    if (whole) {
+      float4* p4 = reinterpret_cast<float4*>(p);
+      float4 a = make_float4(v[0], v[1], v[2], v[3]), b = make_float4(v[4], v[5], v[6], v[7]);
+      if (g.accumulate) {
+        const float4 x = p4[0], y = p4[1];
+        a = make_float4(x.x + a.x, x.y + a.y, x.z + a.z, x.w + a.w);
+        b = make_float4(y.x + b.x, y.y + b.y, y.z + b.z, y.w + b.w);
+      }
+      p4[0] = a;
+      p4[1] = b;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < g.N) p[i] = g.accumulate ? p[i] + v[i] : v[i];
+    }
   } else {
-    static_cast<__nv_bfloat16*>(g.C)[m * g.ldc + n] = __float2bfloat16(v + bias);
+    __nv_bfloat16* p = static_cast<__nv_bfloat16*>(g.C) + at;
+    if (whole) {
+      *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < g.N) p[i] = __float2bfloat16(v[i]);
+    }
   }
 }
 
@@ -219,11 +254,10 @@ __global__ void __launch_bounds__(kThreads1, 2)
       if (!ok) report_status(g.status, kStatusTimeoutEpilogue);
       tc_fence_after();
     }
-    const int n = n0 + q * 32 + lane;
-    const float bias = g.bias != nullptr && n < g.N ? __bfloat162float(g.bias[n]) : 0.f;
+    // sums to shared memory, [row of A][column of C], where the operands lay
     float* part = reinterpret_cast<float*>(smem);
 #pragma unroll 1
-    for (int c = 0; c < TN / 16; ++c) {
+    for (int c = 0; c < TN / 16 && m0 + 16 * c < g.M; ++c) {
       uint32_t r[16];
       if (kb1 > kb0 && ok) {
         tmem_ld_32x32b_x16(tmem + lanes + 16 * c, r);
@@ -232,33 +266,36 @@ __global__ void __launch_bounds__(kThreads1, 2)
 #pragma unroll
         for (int j = 0; j < 16; ++j) r[j] = 0u;
       }
-      if (splits > 1) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) part[(16 * c + j) * kBP + q * 32 + lane] = __uint_as_float(r[j]);
-      } else if (n < g.N) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (m0 + 16 * c + j < g.M) store_c(g, m0 + 16 * c + j, n, __uint_as_float(r[j]), bias);
-      }
+      for (int j = 0; j < 16; ++j) part[(16 * c + j) * kBP + q * 32 + lane] = __uint_as_float(r[j]);
     }
     tc_fence_before();
   }
-  if (splits > 1) {
+  if (splits > 1)
     cluster_sync_block();
-    if (warp >= 2) {
-      const int p = (warp & 3) * 32 + lane, n = n0 + p;
-      if (n < g.N) {
-        const float bias = g.bias != nullptr ? __bfloat162float(g.bias[n]) : 0.f;
-        for (int j = rank; j < TN && m0 + j < g.M; j += splits) {
-          const uint32_t at = smem_u32(smem) + (j * kBP + p) * 4;
-          float v = 0.f;
-          for (int s = 0; s < splits; ++s) v += ld_cluster_f32(at, s);
-          store_c(g, m0 + j, n, v, bias);
-        }
-      }
+  else
+    __syncthreads();
+  // rank r of the cluster adds and stores every splits-th row from r on, eight columns a thread
+  for (int i = threadIdx.x; i < TN / splits * (kBP / 8); i += kThreads1) {
+    const int j = rank + i / (kBP / 8) * splits, n = n0 + i % (kBP / 8) * 8;
+    if (m0 + j >= g.M) break;
+    if (n >= g.N) continue;
+    const uint32_t at = smem_u32(smem) + (j * kBP + i % (kBP / 8) * 8) * 4;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+      const float4 a = ld_cluster_f4(at, s), b = ld_cluster_f4(at + 16, s);
+      v[0] += a.x;
+      v[1] += a.y;
+      v[2] += a.z;
+      v[3] += a.w;
+      v[4] += b.x;
+      v[5] += b.y;
+      v[6] += b.z;
+      v[7] += b.w;
     }
-    cluster_sync_block();   // nobody's sums go before they are read
+    store_c8(g, m0 + j, n, v);
   }
+  if (splits > 1) cluster_sync_block();   // nobody's sums go before they are read
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, F::kCols);
 }
@@ -305,6 +342,7 @@ int block_gemm_1cta(int tn, int splits, const BlockMat& A, const BlockMat& B, vo
   g.b_e5m2 = B.e5m2 ? 1 : 0;
   g.q_rows = M < tn ? M : tn;
   g.tiles_m = (M + tn - 1) / tn;
+  g.vec = !(ldc & 7) && !(reinterpret_cast<uintptr_t>(C) & 15);
   g.status = status;
   const long long tiles = 1LL * g.tiles_m * ((N + kBP - 1) / kBP);
   if (tiles * splits > 0x7fffffffLL) return -3;
@@ -322,14 +360,58 @@ int block_gemm_1cta(int tn, int splits, const BlockMat& A, const BlockMat& B, vo
   return -5;
 }
 
-BlockPlan block_plan(int M, int N, int K, int out_fp32, int accumulate, bool bias, bool aligned) {
-  if (aligned && 1LL * ((M + 255) / 256) * ((N + 255) / 256) >= 40) return BlockPlan{1, 0, 1};
-  const int tn = M <= 16 ? 16 : (M <= 32 ? 32 : (M <= 64 ? 64 : 128));
-  const long long tiles = 1LL * ((M + tn - 1) / tn) * ((N + kBP - 1) / kBP);
+// Modelled time (us) of a product, fitted to 1300 runs of 100 sizes (rows 1 to 6144, columns 768 to 19456, depths 257
+// to 9728, every tile and split that fits, with what a launch costs in a CUDA graph): off by 17 % in the mean for the
+// one-CTA kernel, by 6 % for the pairs; the variant it chooses takes 1.5 % longer than the best in the mean and 19 % at
+// most. Measured at what the choice turns on: 128 x 2304 x 768 5.0 us in tiles of 16, 7.9 on pairs; 128 x 19456 x 2560
+// 17.8 in tiles of 128, 36.9 of 16; 12 x 2560 x 9728 10.1 split four ways, 19.4 whole; 1000 x 4096 x 2560 13.7 on
+// pairs, 16.2 in tiles of 128; 768 x 1152 x 8191 17.3 on pairs split four ways, 25 whole.
+static float cost_1cta(int M, int N, int K, int tn, int splits) {
+  // launch, set-up and epilogue; 1000 deep of one CTA on an SM; of one of two
+  constexpr float kSet[4] = {3.6f, 4.1f, 6.2f, 8.2f}, kOne[4] = {1.67f, 1.77f, 1.85f, 2.36f},
+                  kTwo[4] = {1.29f, 1.56f, 1.47f, 2.14f};
+  const int i = tn == 16 ? 0 : (tn == 32 ? 1 : (tn == 64 ? 2 : 3));
+  const float ctas = 1.f * ((M + tn - 1) / tn) * ((N + kBP - 1) / kBP) * splits;
+  const float depth = 1e-3f * K / splits, waves = ceilf(ctas / 296.f);
+  const float body = fmaxf(kOne[i] * depth * waves, kTwo[i] * depth * ceilf(ctas / 148.f));
+  const float t = kSet[i] * (0.5f + 0.5f * waves) + body + (splits > 1 ? 0.56f * splits : 0.f);
+  return fmaxf(t, 4.8f + 0.2e-6f * N * float(K));   // what memory takes for the weights
+}
+// (The plan depends on the sizes alone, not on the device's count of pairs: storage is sized by it, and it fixes the
+// order of sums.)
+static float cost_2cta(int M, int N, int K, int splits) {
+  constexpr float pairs = 74.f;
+  const float tiles = 1.f * ((M + 255) / 256) * ((N + 255) / 256) * splits;
+  const float each = 1e-3f * K / splits;
+  return 4.85f + ceilf(tiles / pairs) * (1.83f + 2.4f * each) +
+         (splits > 1 ? 3.35f + 0.6e-6f * splits * M * float(N) : 0.f);
+}
+
+BlockPlan block_plan(int M, int N, int K, bool aligned) {
+  BlockPlan best{0, 128, 1, 0.f};
+  best.cost = cost_1cta(M, N, K, 128, 1);
   const int kb = (K + kScaleBlock - 1) / kScaleBlock;
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 2 * 148 && kb >= 4 * splits) splits *= 2;
-  return BlockPlan{0, tn, splits};
+  for (int tn = 16; tn <= 128; tn *= 2) {
+    if (tn >= 32 && tn >= 2 * M) break;
+    for (int s = 1; s <= 8 && s <= kb; s *= 2) {
+      const float c = cost_1cta(M, N, K, tn, s);
+      if (c < best.cost) best = BlockPlan{0, tn, s, c};
+    }
+  }
+  if (!aligned) return best;
+  for (int s = 1; s <= 8; ++s) {
+    if (!block_2cta_splits_ok(K, s)) continue;
+    const float c = cost_2cta(M, N, K, s);
+    if (c < best.cost) best = BlockPlan{1, 0, s, c};
+  }
+  return best;
+}
+
+// The fused projection and activation on CTA pairs, or the products and a launch that activates and casts
+// (measured at 24 x 9728 x 2560: 25.8 and 17.0 us; 500 x 4096 x 1024: 13.5 and 15.5).
+bool block_glu_fused(int T, int I, int K) {
+  const float fused = cost_2cta(T, 2 * I, K, 1) + 1.f;
+  return fused < block_plan(T, 2 * I, K, true).cost + 2.5f + 2e-6f * T * float(I);
 }
 
 size_t block_plan_bytes(const BlockPlan& p, int M, int N) {
@@ -358,11 +440,10 @@ bool aligned_for_pairs(const void* C, int N, long long ldc) {
 }  // namespace
 
 // Bytes of temporary storage that lb_gemm_block wants for this product (a 16-byte aligned C).
-extern "C" long long lb_gemm_block_bytes(int M, int N, int K, long long ldc, int out_fp32, int accumulate,
-                                         int bias) {
+extern "C" long long lb_gemm_block_bytes(int M, int N, int K, long long ldc) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   return (long long)lb::block_plan_bytes(
-      lb::block_plan(M, N, K, out_fp32, accumulate, bias != 0, aligned_for_pairs(nullptr, N, ldc)), M, N);
+      lb::block_plan(M, N, K, aligned_for_pairs(nullptr, N, ldc)), M, N);
 }
 
 // C [M, N] (bf16 or fp32, rows ldc elements apart) = A · Bᵀ + bias for A [M, K] and B [N, K] in 8 bits
@@ -379,7 +460,7 @@ extern "C" int lb_gemm_block(const void* A, const void* B, void* C, int M, int N
   if (accumulate && (!out_fp32 || bias != nullptr)) return -5;
   const BlockMat a{(uint8_t*)A, lda, (uint32_t*)sa, rows_sa, a_e5m2};
   const BlockMat b{(uint8_t*)B, ldb, (uint32_t*)sb, rows_sb, b_e5m2};
-  const BlockPlan p = block_plan(M, N, K, out_fp32, accumulate, bias != nullptr, aligned_for_pairs(C, N, ldc));
+  const BlockPlan p = block_plan(M, N, K, aligned_for_pairs(C, N, ldc));
   if (block_plan_bytes(p, M, N) > size_t(ws_bytes)) return -6;
   return block_gemm(p, a, b, C, M, N, K, ldc, out_fp32, accumulate, bias, ws, status,
                     reinterpret_cast<cudaStream_t>(stream_));

@@ -19,8 +19,8 @@
 #include "../common/pdl.h"
 #include "../common/ptx.cuh"
 #include "../common/tma_desc.h"
-#include "../row/glu.cuh"
 #include "block_gemm.h"
+#include "block_glu.cuh"
 #include "block_scale.cuh"
 
 namespace lb {
@@ -334,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const uint4 v = glu_fwd8<GLU - 1>(
+            const uint4 v = block_glu8<GLU - 1>(
                 make_uint4(w[0][4 * j], w[0][4 * j + 1], w[0][4 * j + 2], w[0][4 * j + 3]),
                 make_uint4(w[1][4 * j], w[1][4 * j + 1], w[1][4 * j + 2], w[1][4 * j + 3]));
             h[i][4 * j] = v.x;
@@ -376,9 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         *tops = top;
         asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
         top = max(top, tops[half ? -4 * EPI_WORDS : 4 * EPI_WORDS]);   // the warp with the other half of the rows
-        const uint32_t e = block_scale_byte<0>(top);
-        const bool fine = block_is_finite(top);
-        const float s = block_inverse(e);
+        const float s = block_inverse<0>(top);
         if (row < g.M) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -387,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const float2 a = unpack_bf16x2(h[i][2 * j]), b = unpack_bf16x2(h[i][2 * j + 1]);
-              o[j] = fine ? cast4<0>(a.x * s, a.y * s, b.x * s, b.y * s) : 0x7f7f7f7fu;
+              o[j] = cast4<0>(a.x * s, a.y * s, b.x * s, b.y * s);
             }
             uint4* dst = reinterpret_cast<uint4*>(g.h + row * g.ldh + f0);
             dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
@@ -396,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (half == 0) {
             const int kb = n0 / kScaleBlock;
             uint8_t* p = reinterpret_cast<uint8_t*>(g.h_scales + (kb >> 2) * g.rows_h + row);
-            p[kb & 3] = uint8_t(fine ? e : kScaleOne);
+            p[kb & 3] = uint8_t(block_scale_byte<0>(top));
             if (n0 + kScaleBlock >= g.N)
               for (int k = (kb & 3) + 1; k < 4; ++k) p[k] = uint8_t(kScaleOne);
           }
@@ -532,15 +530,6 @@ int stages_of_split(int K, int splits) {
 bool block_2cta_splits_ok(int K, int splits) {
   const int stages = (K + BK - 1) / BK, each = stages_of_split(K, splits);
   return (stages + each - 1) / each == splits;
-}
-
-// Asks the driver with the first product's launch; half the SMs before that.
-int block_2cta_pairs() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 74;
-  if (g_pairs[dev] > 0) return g_pairs[dev];
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms / 2;
 }
 
 // N a multiple of 8, C 16-byte aligned, ldc a multiple of 8. splits > 1 (fp32): split s of the contraction writes its

@@ -20,7 +20,6 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
-from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -31,26 +30,50 @@ from .activation import glu_ref
 from ._grads import main_grad_of
 
 BLOCK = 128
-E4M3_MAX, E5M2_MAX = 448.0, 57344.0
+_MOST = 1 << 30      # rows and columns are counted in 32 bits
 
 
-@dataclass
 class Fp8BlockTensor:
     """A matrix ``[rows, cols]`` in 8 bits: ``data`` ``[rows, ld]`` bytes (the first ``cols`` of a row are
     valid; ``ld`` a multiple of 16), ``scales`` ``[ceil(cols / 512), rows, 4]`` bytes: ``scales[b // 4, r,
-    b % 4]`` is the exponent, biased by 127, of the scale of columns ``128 b .. 128 b + 127`` of row ``r``."""
-    data: torch.Tensor
-    cols: int
-    scales: torch.Tensor
-    e5m2: bool = False
+    b % 4]`` is the exponent, biased by 127, of the scale of columns ``128 b .. 128 b + 127`` of row ``r``.
 
-    @property
-    def rows(self) -> int:
-        return self.data.shape[0]
+    The two are checked here, once; a product takes them as they are.
+    """
+    __slots__ = ("_data", "_cols", "_scales", "_e5m2", "_where")
 
-    @property
-    def shape(self):
-        return (self.data.shape[0], self.cols)
+    def __init__(self, data: torch.Tensor, cols: int, scales: torch.Tensor, e5m2: bool = False):
+        if data.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or data.dim() != 2 or scales.dim() != 3:
+            raise TypeError("data is a 2-D and scales a 3-D tensor of bytes")
+        (rows, width), (ld, step) = data.shape, data.stride()
+        groups, s_rows, four = scales.shape
+        s_group, s_row, s_byte = scales.stride()
+        if not 0 <= cols <= width or groups != (cols + 511) // 512 or s_rows != rows or four != 4:
+            raise ValueError(f"data {tuple(data.shape)} with {cols} columns and scales {tuple(scales.shape)} do not "
+                             f"belong together")
+        if rows <= 1:       # strides of a dimension of one say nothing
+            ld, s_row = (width + 15) // 16 * 16, 4
+        if groups <= 1:
+            s_group = 4 * rows
+        if width and rows and ((step != 1 and width > 1) or ld < cols):
+            raise ValueError("the bytes of a row lie next to one another")
+        if rows and groups and (s_byte != 1 or s_row != 4 or s_group % 4 or s_group < 4 * rows):
+            raise ValueError("the scales of four blocks lie next to one another, row by row")
+        ptr, s_ptr = data.data_ptr(), scales.data_ptr()
+        if data.is_cuda and (ld % 16 or ptr % 16 or s_ptr % 4) and width and rows:
+            raise ValueError("rows start at multiples of 16 bytes, their scales at multiples of 4")
+        if data.get_device() != scales.get_device():
+            raise ValueError("data and scales are on one device")
+        self._data, self._cols, self._scales, self._e5m2 = data, cols, scales, bool(e5m2)
+        # as the launchers take it: bytes, their row stride, scale words, words of a group of four blocks
+        self._where = (ptr, ld, s_ptr, s_group // 4)
+
+    data = property(lambda self: self._data)
+    cols = property(lambda self: self._cols)
+    scales = property(lambda self: self._scales)
+    e5m2 = property(lambda self: self._e5m2)
+    rows = property(lambda self: self._data.shape[0])
+    shape = property(lambda self: (self._data.shape[0], self._cols))
 
     def dequantize(self) -> torch.Tensor:
         """The values, in fp32."""
@@ -59,32 +82,6 @@ class Fp8BlockTensor:
         s = (e << 23).view(torch.float32).repeat_interleave(BLOCK, dim=1)[:, :self.cols]
         return q.float() * s
 
-    def check(self, what: str) -> None:
-        d, s = self.data, self.scales
-        if d.dim() != 2 or d.dtype != torch.uint8 or s.dim() != 3 or s.dtype != torch.uint8:
-            raise TypeError(f"{what}: data is a 2-D and scales a 3-D tensor of bytes")
-        if not 0 <= self.cols <= d.shape[1] or tuple(s.shape) != (-(-self.cols // 512), d.shape[0], 4):
-            raise ValueError(f"{what}: data {tuple(d.shape)} with {self.cols} columns and scales "
-                             f"{tuple(s.shape)} do not belong together")
-        if (d.stride(1) != 1 and d.shape[1] > 1) or (d.shape[0] > 1 and d.stride(0) < self.cols):
-            raise ValueError(f"{what}: the bytes of a row lie next to one another")
-        if d.is_cuda and d.numel() and (_row_bytes(d) % 16 or d.data_ptr() % 16):
-            raise ValueError(f"{what}: rows start at multiples of 16 bytes")
-        if not s[0].is_contiguous() if s.shape[0] else False:
-            raise ValueError(f"{what}: the scales of four blocks lie next to one another, row by row")
-        if s.device != d.device:
-            raise ValueError(f"{what}: data and scales are on one device")
-
-
-def _row_bytes(d: torch.Tensor) -> int:
-    """Bytes between two rows (of a single row: enough of them)."""
-    return d.stride(0) if d.shape[0] > 1 else (d.shape[1] + 15) // 16 * 16
-
-
-def _scale_rows(s: torch.Tensor) -> int:
-    """Words between the scales of one group of four blocks and the next."""
-    return s.stride(0) // 4 if s.shape[0] > 1 else s.shape[1]
-
 
 # ------------------------------------------------------------------------------------------------
 # Calls into the library
@@ -92,14 +89,14 @@ def _scale_rows(s: torch.Tensor) -> int:
 _P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 _SIGNATURES = {
     "lb_block_cast": [_P, _I, _I, _L, _I, _I, _P, _L, _P, _L, _P, _L, _P, _L, _I, _P],
-    "lb_gemm_block_bytes": [_I, _I, _I, _L, _I, _I, _I],
+    "lb_gemm_block_bytes": [_I, _I, _I, _L],
     "lb_gemm_block": [_P, _P, _P, _I, _I, _I, _L, _L, _L, _I, _I, _P, _L, _P, _L, _I, _I, _P, _P, _L, _P, _P],
-    "lb_linear_block_bytes": [_I] * 6 + [_P],
+    "lb_linear_block_bytes": [_I] * 4 + [_P],
     "lb_linear_block_fwd": [_P, _L, _P, _L, _P, _I, _I, _I, _I, _I] + [_P] * 5,
     "lb_linear_block_bwd": [_P, _L, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _P, _I, _P, _P],
-    "lb_linear_kept_bytes": [_I] * 4,
+    "lb_linear_kept_bytes": [_I] * 3,
     "lb_linear_kept_fwd": [_P, _L, _P, _L, _P, _L, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P],
-    "lb_mlp_block_bytes": [_I] * 4 + [_P, _P],
+    "lb_mlp_block_bytes": [_I] * 4 + [_P],
     "lb_mlp_block_fwd": [_I, _P, _L, _P, _L, _P, _L, _P, _L, _I, _I, _I, _I] + [_P] * 5,
     "lb_mlp_block_bwd": [_I, _P, _L, _I, _I, _I, _I, _I] + [_P] * 9,
     "lb_mlp_kept_bytes": [_I] * 3,
@@ -125,18 +122,28 @@ def _call(name, *args):
         nv.check_rc(rc, f"{name}{tuple(a for a in args if a is not None and not a >> 24)}")
 
 
-def _on_device(*tensors):
-    """The tensors' one CUDA device as a context: launches go to the current stream of that device."""
-    dev = None
-    for t in tensors:
-        if t is not None:
-            if dev is not None and t.device != dev:
-                raise ValueError(f"operands are on {dev} and {t.device}")
-            dev = t.device
-    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
 _HERE = contextlib.nullcontext()
+
+
+def _on_device(first, *others):
+    """The tensors' one CUDA device as a context: launches go to the current stream of that device."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"operands are on {first.device} and {t.device}")
+    return _HERE if dev == _current_device() else torch.cuda.device(dev)
+
+
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+_status = {}
+
+
+def _status_ptr(device) -> int:
+    """Address of the device's status word, which stays where it is."""
+    p = _status.get(device.index)
+    if p is None:
+        p = _status[device.index] = nv.status_word(device).data_ptr()
+    return p
 
 
 def _bytes(n: int, device) -> torch.Tensor:
@@ -202,18 +209,19 @@ def _empty(rows, cols, e5m2, device) -> Fp8BlockTensor:
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
     """``x`` [R, C] in bf16 with rows that a kernel can read in 16-byte pieces."""
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not torch.bfloat16:
         x = x.to(torch.bfloat16)
-    if x.stride(1) != 1 or x.stride(0) % 8 or x.stride(0) < x.shape[1] or x.data_ptr() % 16:
+    ld, step = x.stride()
+    if step != 1 or ld % 8 or ld < x.shape[1] or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
-def _where(q: Optional[Fp8BlockTensor]):
-    """A cast matrix as the launchers take it: bytes, their row stride, scale words, words of a group."""
-    if q is None:
-        return 0, 0, 0, 0
-    return q.data.data_ptr(), _row_bytes(q.data), q.scales.data_ptr(), _scale_rows(q.scales)
+def _rows(x: torch.Tensor, width: int) -> torch.Tensor:
+    return x if x.dim() == 2 else x.reshape(-1, width)
+
+
+_NONE = (0, 0, 0, 0)
 
 
 def quantize_fp8_block(x: torch.Tensor, *, tile: bool = False, e5m2: bool = False, want: bool = True,
@@ -232,13 +240,15 @@ def quantize_fp8_block(x: torch.Tensor, *, tile: bool = False, e5m2: bool = Fals
     R, C = x.shape
     if C % 8:
         raise ValueError("quantize_fp8_block needs a multiple of 8 columns")
+    if R >= _MOST or C >= _MOST:
+        raise ValueError(f"more rows or columns than the kernels count: {R}, {C}")
     with _on_device(x):
         x = _aligned(x.detach())
         out = _empty(R, C, e5m2, x.device) if want else None
         out_t = _empty(C, R, e5m2, x.device) if want_t else None
         if R and C and (want or want_t):
-            _call("lb_block_cast", x.data_ptr(), R, C, x.stride(0), tile, e5m2, *_where(out), *_where(out_t), 0,
-                  nv.stream_ptr())
+            _call("lb_block_cast", x.data_ptr(), R, C, x.stride(0), tile, e5m2, *(out._where if want else _NONE),
+                  *(out_t._where if want_t else _NONE), 0, nv.stream_ptr())
             nv.count_launch()
     return out, out_t
 
@@ -247,8 +257,8 @@ def quantize_fp8_block(x: torch.Tensor, *, tile: bool = False, e5m2: bool = Fals
 # Products
 # ------------------------------------------------------------------------------------------------
 @functools.lru_cache(maxsize=4096)
-def _product_bytes(M, N, K, ldc, fp32, accumulate, bias) -> int:
-    return _fn("lb_gemm_block_bytes")(M, N, K, ldc, fp32, accumulate, bias)
+def _product_bytes(M, N, K, ldc) -> int:
+    return _fn("lb_gemm_block_bytes")(M, N, K, ldc)
 
 
 def matmul_fp8_block(a: Fp8BlockTensor, b: Fp8BlockTensor, *, out: Optional[torch.Tensor] = None,
@@ -258,8 +268,6 @@ def matmul_fp8_block(a: Fp8BlockTensor, b: Fp8BlockTensor, *, out: Optional[torc
     ``out`` may be given (rows of unit inner stride); ``accumulate`` adds into it (fp32, no bias). Sums are
     fp32 and their order depends on the sizes alone. e4m3 and e5m2 operands may be mixed.
     """
-    a.check("a")
-    b.check("b")
     M, N, K = a.rows, b.rows, a.cols
     if b.cols != K:
         raise ValueError(f"contraction mismatch: {K} vs {b.cols}")
@@ -292,12 +300,11 @@ def matmul_fp8_block(a: Fp8BlockTensor, b: Fp8BlockTensor, *, out: Optional[torc
         if bias is not None:
             bias = bias.to(torch.bfloat16).contiguous()
         ldc, fp32 = (out.stride(0) if M > 1 else N), out_dtype == torch.float32
-        n = _product_bytes(M, N, K, ldc, fp32, accumulate, bias is not None)
+        n = _product_bytes(M, N, K, ldc)
         ws = _bytes(n, out.device) if n else None
-        _call("lb_gemm_block", a.data.data_ptr(), b.data.data_ptr(), out.data_ptr(), M, N, K, _row_bytes(a.data),
-              _row_bytes(b.data), ldc, a.e5m2, b.e5m2, a.scales.data_ptr(), _scale_rows(a.scales), b.scales.data_ptr(),
-              _scale_rows(b.scales), fp32, accumulate, nv.ptr(bias), nv.ptr(ws), n,
-              nv.status_word(out.device).data_ptr(), nv.stream_ptr())
+        (pa, lda, sa, rows_a), (pb, ldb, sb, rows_b) = a._where, b._where
+        _call("lb_gemm_block", pa, pb, out.data_ptr(), M, N, K, lda, ldb, ldc, a.e5m2, b.e5m2, sa, rows_a, sb, rows_b, fp32,
+              accumulate, nv.ptr(bias), nv.ptr(ws), n, _status_ptr(out.device), nv.stream_ptr())
         nv.count_launch()
     return out
 
@@ -334,20 +341,22 @@ def _returned(w, out):
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear_bytes(T, K, N, need, y_mode, dw_mode):
+def _linear_bytes(T, K, N, need):
     out = (_L * 3)()
-    _fn("lb_linear_block_bytes")(T, K, N, need, y_mode, dw_mode, ctypes.addressof(out))
+    _fn("lb_linear_block_bytes")(T, K, N, need, ctypes.addressof(out))
     return tuple(out)
 
 
 @functools.lru_cache(maxsize=4096)
-def _linear_kept_bytes(T, K, N, y_mode):
-    return _fn("lb_linear_kept_bytes")(T, K, N, y_mode)
+def _linear_kept_bytes(T, K, N):
+    return _fn("lb_linear_kept_bytes")(T, K, N)
 
 
-def _check_widths(*widths):
-    if any(n % 8 for n in widths):
-        raise ValueError(f"block-scaled layers need multiples of 8 features, got {widths}")
+def _check_widths(T, K, N=0):
+    if K % 8 or N % 8:
+        raise ValueError(f"block-scaled layers need multiples of 8 features, got {K} and {N}")
+    if T >= _MOST or K >= _MOST or N >= _MOST:
+        raise ValueError(f"more rows or columns than the kernels count: {T}, {K}, {N}")
 
 
 class _LinearFp8Block(torch.autograd.Function):
@@ -356,29 +365,29 @@ class _LinearFp8Block(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w, bias):
-        x2 = x.reshape(-1, x.shape[-1])
+        x2 = _rows(x, x.shape[-1])
         T, K = x2.shape
         N = w.shape[0]
         ctx.need = need = ctx.needs_input_grad[0] + 2 * ctx.needs_input_grad[1] + 4 * ctx.needs_input_grad[2]
         ctx.x_like = (x.shape, x.dtype)
         ctx.bias_dtype = None if bias is None else bias.dtype
         act = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
-        if not nv.use_native(x, w, bias):
+        if not x.is_cuda:
             xq, xq_t = _quantize_eager(x2, False, False, True, True)
             wq, _ = _quantize_eager(w, True, False, True, False)
             ctx.save_for_backward(w, xq_t.dequantize(), wq.dequantize())
             return matmul_fp8_block(xq, wq, out_dtype=act, bias=bias).view(*x.shape[:-1], N)
-        _check_widths(K, N)
+        _check_widths(T, K, N)
         with _on_device(x, w, bias):
             x2, w2 = _aligned(x2), _aligned(w)
             if bias is not None:
                 bias = bias.to(torch.bfloat16).contiguous()
-            n_saved, n_tmp, _ = _linear_bytes(T, K, N, need, _mode(act), _BF16)
+            n_saved, n_tmp, _ = _linear_bytes(T, K, N, need)
             saved, tmp = _bytes(n_saved, x.device), _bytes(n_tmp, x.device)
             y = torch.empty(*x.shape[:-1], N, dtype=act, device=x.device)
             _call("lb_linear_block_fwd", x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), nv.ptr(bias), T, K, N,
                   need, _mode(act), y.data_ptr(), saved.data_ptr(), tmp.data_ptr(),
-                  nv.status_word(x.device).data_ptr(), nv.stream_ptr())
+                  _status_ptr(x.device), nv.stream_ptr())
             nv.count_launch(3)
         ctx.save_for_backward(w, saved)
         return y
@@ -389,7 +398,7 @@ class _LinearFp8Block(torch.autograd.Function):
         w = ctx.saved_tensors[0]
         shape, x_dtype = ctx.x_like
         N, K = w.shape
-        dy2 = dy.reshape(-1, N)
+        dy2 = _rows(dy, N)
         T, need = dy2.shape[0], ctx.need
         dx = dw = db = None
         if len(ctx.saved_tensors) == 3:      # on the CPU
@@ -413,10 +422,10 @@ class _LinearFp8Block(torch.autograd.Function):
                 db = torch.empty(N, dtype=torch.bfloat16 if ctx.bias_dtype == torch.bfloat16 else torch.float32,
                                  device=dy.device)
             x_mode = _FP32 if dx is not None and dx.dtype == torch.float32 else _BF16
-            tmp = _bytes(_linear_bytes(T, K, N, need, x_mode, g[1])[2], dy.device)
+            tmp = _bytes(_linear_bytes(T, K, N, need)[2], dy.device)
             _call("lb_linear_block_bwd", dy2.data_ptr(), dy2.stride(0), T, K, N, need, saved.data_ptr(), tmp.data_ptr(),
                   nv.ptr(dx), x_mode, nv.ptr(g[0]), g[1], nv.ptr(db), 0 if db is None else _mode(db.dtype),
-                  nv.status_word(dy.device).data_ptr(), nv.stream_ptr())
+                  _status_ptr(dy.device), nv.stream_ptr())
             nv.count_launch(1 + bool(need & 1) + bool(need & 2) + bool(need & 4))
             dw = _returned(w, g[0]) if need & 2 else None
             return (None if dx is None else dx.to(x_dtype)), dw, (None if db is None else db.to(ctx.bias_dtype))
@@ -442,26 +451,26 @@ def linear_fp8_block(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) ->
         if not torch.is_grad_enabled():      # nothing is kept for a backward then
             x, w, bias = x.detach(), w.detach(), None if bias is None else bias.detach()
         return _LinearFp8Block.apply(x, w, bias)
-    w.check("w")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("a kept 8-bit weight is for passes without gradients")
-    act = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
-    x2 = x.reshape(-1, K)
-    if x2.numel() == 0 or N == 0 or not nv.use_native(x, w.data, bias):
+    fp32 = x.dtype is torch.float32
+    act = torch.float32 if fp32 else torch.bfloat16
+    x2 = _rows(x, K)
+    T = x2.shape[0]
+    if T * K * N == 0 or not (x.is_cuda and w._data.is_cuda):
         xq, _ = quantize_fp8_block(x2)
         return matmul_fp8_block(xq, w, out_dtype=act, bias=bias).view(*x.shape[:-1], N)
-    _check_widths(K, N)
-    with _on_device(x, w.data, bias):
+    _check_widths(T, K, N)
+    with _on_device(x, w._data, bias):
         x2 = _aligned(x2)
         if bias is not None:
             bias = bias.to(torch.bfloat16).contiguous()
-        T, mode = x2.shape[0], _mode(act)
-        y = torch.empty(*x.shape[:-1], N, dtype=act, device=x.device)
-        tmp = _bytes(_linear_kept_bytes(T, K, N, mode), x.device)
-        _call("lb_linear_kept_fwd", x2.data_ptr(), x2.stride(0), *_where(w), w.e5m2, nv.ptr(bias), T, K, N, mode,
-              y.data_ptr(), tmp.data_ptr(), nv.status_word(x.device).data_ptr(), nv.stream_ptr())
+        y = torch.empty((T, N), dtype=act, device=x.device)
+        tmp = _bytes(_linear_kept_bytes(T, K, N), x.device)
+        _call("lb_linear_kept_fwd", x2.data_ptr(), x2.stride(0), *w._where, w._e5m2, nv.ptr(bias), T, K, N, fp32,
+              y.data_ptr(), tmp.data_ptr(), _status_ptr(x.device), nv.stream_ptr())
         nv.count_launch(2)
-    return y
+    return y if x2.dim() == x.dim() else y.view(*x.shape[:-1], N)
 
 
 _KINDS = {"swiglu": 0, "geglu": 1}
@@ -488,9 +497,9 @@ def _mlp_eager(xq, w, wd, kind):
 
 
 @functools.lru_cache(maxsize=4096)
-def _mlp_bytes(T, H, I, need, *modes):
-    out, m = (_L * 3)(), (_I * 3)(*modes)
-    _fn("lb_mlp_block_bytes")(T, H, I, need, ctypes.addressof(m), ctypes.addressof(out))
+def _mlp_bytes(T, H, I, need):
+    out = (_L * 3)()
+    _fn("lb_mlp_block_bytes")(T, H, I, need, ctypes.addressof(out))
     return tuple(out)
 
 
@@ -506,29 +515,29 @@ class _GatedMlpFp8Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, kind):
         H, I = w_down.shape
-        x2 = x.reshape(-1, H)
+        x2 = _rows(x, H)
         T = x2.shape[0]
         nx, ng, nu, nd = ctx.needs_input_grad[:4]
         ctx.need = need = nx + 2 * (ng or nu) + 4 * nd
         ctx.kind, ctx.x_like = kind, (x.shape, x.dtype)
         act = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
-        if not nv.use_native(x, w_gate, w_up, w_down):
+        if not x.is_cuda:
             xq, xq_t = _quantize_eager(x2, False, False, True, True)
             w = w_gate if w_up is None else torch.cat([w_gate, w_up])
             wq, dq = (_quantize_eager(t, True, False, True, False)[0] for t in (w, w_down))
             gu, h, y = _mlp_eager(xq, wq, dq, kind)
             ctx.save_for_backward(w_gate, w_up, w_down, gu, h, xq_t.dequantize(), wq.dequantize(), dq.dequantize())
             return y.view(x.shape).to(act)
-        _check_widths(H)
+        _check_widths(T, H, I)
         with _on_device(x, w_gate, w_up, w_down):
             x2, wg, wd = _aligned(x2), _aligned(w_gate), _aligned(w_down)
             wu = None if w_up is None else _aligned(w_up)
-            n_saved, n_tmp, _ = _mlp_bytes(T, H, I, need, 0, 0, 0)
+            n_saved, n_tmp, _ = _mlp_bytes(T, H, I, need)
             saved, tmp = _bytes(n_saved, x.device), _bytes(n_tmp, x.device)
             y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
             _call("lb_mlp_block_fwd", _KINDS[kind], x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), nv.ptr(wu),
                   0 if wu is None else wu.stride(0), wd.data_ptr(), wd.stride(0), T, H, I, need, y.data_ptr(),
-                  saved.data_ptr(), tmp.data_ptr(), nv.status_word(x.device).data_ptr(), nv.stream_ptr())
+                  saved.data_ptr(), tmp.data_ptr(), _status_ptr(x.device), nv.stream_ptr())
             nv.count_launch(5 + (wu is not None))
         ctx.save_for_backward(w_gate, w_up, w_down, saved)
         return y.to(act)
@@ -539,7 +548,7 @@ class _GatedMlpFp8Block(torch.autograd.Function):
         w_gate, w_up, w_down = ctx.saved_tensors[:3]
         shape, x_dtype = ctx.x_like
         H, I = w_down.shape
-        dy2 = dy.reshape(-1, H)
+        dy2 = _rows(dy, H)
         T, need = dy2.shape[0], ctx.need
         nx, ng, nu, nd = ctx.needs_input_grad[:4]
         dx = dg = du = dd = None
@@ -567,11 +576,11 @@ class _GatedMlpFp8Block(torch.autograd.Function):
             grads = [_gradient_of(w) if n else (None, _BF16)
                      for w, n in ((w_gate, ng), (w_up, nu), (w_down, nd))]
             modes = [g[1] for g in grads]
-            tmp = _bytes(_mlp_bytes(T, H, I, need, *modes)[2], dy.device)
+            tmp = _bytes(_mlp_bytes(T, H, I, need)[2], dy.device)
             m = (_I * 3)(*modes)
             _call("lb_mlp_block_bwd", _KINDS[ctx.kind], dy2.data_ptr(), dy2.stride(0), T, H, I, need, w_up is None,
                   saved.data_ptr(), tmp.data_ptr(), nv.ptr(dx), *(nv.ptr(g[0]) for g in grads), ctypes.addressof(m),
-                  nv.status_word(dy.device).data_ptr(), nv.stream_ptr())
+                  _status_ptr(dy.device), nv.stream_ptr())
             nv.count_launch(2 + bool(need & 3) + nx + ng + nu + nd)
             dg, du, dd = (_returned(w, g[0]) if n else None
                           for w, n, g in zip((w_gate, w_up, w_down), (ng, nu, nd), grads))
@@ -611,25 +620,23 @@ def gated_mlp_fp8_block(x: torch.Tensor, w_gate, w_up, w_down, kind: str = "swig
         return _GatedMlpFp8Block.apply(x, w_gate, w_up, w_down, kind)
     if not (kept[0] and kept[2]) or w_up is not None:
         raise ValueError("8-bit weights come as a fused gate and up weight and a down weight")
-    w_gate.check("w_gate")
-    w_down.check("w_down")
     if torch.is_grad_enabled() and x.requires_grad:
         raise ValueError("a kept 8-bit weight is for passes without gradients")
     act = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
     if x.numel() == 0:
         return torch.empty(x.shape, dtype=act, device=x.device)
-    x2 = x.reshape(-1, H)
-    if not nv.use_native(x, w_gate.data, w_down.data):
+    x2 = _rows(x, H)
+    if not x.is_cuda:
         xq, _ = _quantize_eager(x2, False, False, True, False)
         return _mlp_eager(xq, w_gate, w_down, kind)[2].view(x.shape).to(act)
-    _check_widths(H)
-    with _on_device(x, w_gate.data, w_down.data):
+    T = x2.shape[0]
+    _check_widths(T, H, I)
+    with _on_device(x, w_gate._data, w_down._data):
         x2 = _aligned(x2)
-        T = x2.shape[0]
         y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
         tmp = _bytes(_mlp_kept_bytes(T, H, I), x.device)
-        _call("lb_mlp_kept_fwd", _KINDS[kind], x2.data_ptr(), x2.stride(0), *_where(w_gate), w_gate.e5m2,
-              *_where(w_down), w_down.e5m2, T, H, I, y.data_ptr(), tmp.data_ptr(),
-              nv.status_word(x.device).data_ptr(), nv.stream_ptr())
+        _call("lb_mlp_kept_fwd", _KINDS[kind], x2.data_ptr(), x2.stride(0), *w_gate._where, w_gate._e5m2,
+              *w_down._where, w_down._e5m2, T, H, I, y.data_ptr(), tmp.data_ptr(),
+              _status_ptr(x.device), nv.stream_ptr())
         nv.count_launch(4)
     return y.to(act)
