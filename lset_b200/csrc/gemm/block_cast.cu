@@ -18,6 +18,7 @@ namespace lb {
 namespace {
 
 using bf16 = __nv_bfloat16;
+constexpr int kMaxDevices = 64;
 
 // The bytes of four words of a 4 x 4 block, transposed.
 __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
@@ -50,13 +51,16 @@ __device__ __forceinline__ void store_scale(const BlockOut& o, long long r, int 
 }
 
 constexpr int kTile = 128;
-struct CastSmem {
-  uint32_t tile[kTile * kTile / 4];  // [column][four rows]
-  uint32_t part[16][64];             // a warp's maxima of its 128 columns, two a word
-  uint32_t all[8];
-};
-
 enum { kRows = 1, kCols = 2 };
+
+// Shared memory of A tiles that are cast together.
+template <int A>
+struct CastSmem {
+  uint32_t tile[A][kTile * kTile / 4];   // [column][four rows], bytes of the transposed copies
+  uint32_t part[A][16][64];              // a warp's maxima of its 128 columns, two a word
+  float2 cols[A][64];                    // what the columns are multiplied by
+  uint32_t all[16];
+};
 
 // The 128 x 128 tile at (r0, c0) of a matrix [R, C] that the CTA's 512 / U threads hold in registers: thread
 // (rq, cg) = (threadIdx.x / 16, % 16) has rows rq * 4 + 64 u + i, columns cg * 8 .. cg * 8 + 7 in v[u][i]
@@ -64,145 +68,172 @@ enum { kRows = 1, kCols = 2 };
 // tile; else `out` has one for each row and `out_t` for each column.
 //
 // Magnitudes are compared as integers (bf16 bits without the sign), two at a time, which also lets NaN and
-// infinities through to the top. Bound by issued instructions before memory (4 bytes a value, read and both
-// outputs), so a value is unpacked once for both, scaled two at a time, and a lane stores one scale.
-template <int TILED, int E5M2, int WANT, int U>
-__device__ __forceinline__ void cast_tile(const uint4 (&v)[U][4], CastSmem& sm, int r0, int c0, int R, int C,
-                                          const BlockOut& out, const BlockOut& out_t) {
-  constexpr int kWarps = 16 / U, kMine = 4 * U, kPairs = kMine / 2;   // rows of a thread; row p with p + kPairs a word
-  const int cg = threadIdx.x & 15, rq = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = c0 + cg * 8;
-  constexpr uint32_t kAbs = 0x7fff7fffu;
-  uint32_t col[4] = {0u, 0u, 0u, 0u};   // maxima of the thread's eight columns
-  uint32_t row[kPairs];                 // and of its rows
-  {
-    uint32_t m[kMine];
+// infinities through to the top. Bound by issued instructions before memory, so a value is unpacked once for both
+// layouts and scaled two at a time, a lane stores one scale, and 64 threads join the warps' column maxima for all.
+// The steps of a cast are apart, so that tiles cast together (the gated backward's three) share their barriers:
+// maxima, barrier, join_cols, barrier, write, barrier, copy_cols.
+template <int E5M2, int WANT, int U>
+struct Cast {
+  static constexpr int kWarps = 16 / U, kMine = 4 * U, kPairs = kMine / 2;   // a thread's rows; rows p, p + kPairs a word
+  static constexpr uint32_t kAbs = 0x7fff7fffu;
+
+  // rs: what the thread's rows are multiplied by (their scales are stored); the columns' maxima go to `part`.
+  static __device__ __forceinline__ void maxima(const uint4 (&v)[U][4], uint32_t (&part)[16][64], float (&rs)[kMine],
+                                                int r0, int c0, int R, int C, const BlockOut& out) {
+    const int cg = threadIdx.x & 15, rq = threadIdx.x >> 4, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t col[4] = {0u, 0u, 0u, 0u}, m[kMine];
 #pragma unroll
     for (int p = 0; p < kMine; ++p) {
       const uint4& q = v[p / 4][p % 4];
       const uint32_t w[4] = {q.x & kAbs, q.y & kAbs, q.z & kAbs, q.w & kAbs};
-      if (TILED || (WANT & kCols)) {
+      if (WANT & kCols) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) col[j] = __vmaxu2(col[j], w[j]);
       }
-      if (!TILED && (WANT & kRows)) m[p] = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
-    }
-    if (!TILED && (WANT & kRows)) {
-#pragma unroll
-      for (int p = 0; p < kPairs; ++p)
-        row[p] = __vmaxu2(__byte_perm(m[p], m[p + kPairs], 0x5410), __byte_perm(m[p], m[p + kPairs], 0x7632));
-    }
-  }
-  float rs[kMine];
-  f2 cs[4];
-  if (TILED) {
-    uint32_t m = __vmaxu2(__vmaxu2(col[0], col[1]), __vmaxu2(col[2], col[3]));
-    m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
-    if (lane == 0) sm.all[warp] = m;
-    __syncthreads();
-    m = 0u;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) m = max(m, sm.all[k]);
-    const float s = block_inverse<E5M2>(m);
-    const uint32_t e = block_scale_byte<E5M2>(m);
-    cs[0] = cs[1] = cs[2] = cs[3] = f2_of(s, s);
-    if (threadIdx.x < kTile) {
-      if ((WANT & kRows) && r0 + threadIdx.x < R) store_scale(out, r0 + threadIdx.x, c0 / kTile, c0 + kTile >= C, e);
-      if ((WANT & kCols) && c0 + threadIdx.x < C) store_scale(out_t, c0 + threadIdx.x, r0 / kTile, r0 + kTile >= R, e);
-    }
-  } else {
-    if (WANT & kRows) {
-#pragma unroll
-      for (int p = 0; p < kPairs; ++p) {
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) row[p] = __vmaxu2(row[p], __shfl_xor_sync(0xffffffffu, row[p], o));
-        rs[p] = block_inverse<E5M2>(row[p] & 0xffffu);
-        rs[p + kPairs] = block_inverse<E5M2>(row[p] >> 16);
-      }
-      if (cg < kMine) {   // lane cg stores the scale of row cg of the thread's
-        uint32_t w = row[0];
-#pragma unroll
-        for (int p = 1; p < kPairs; ++p) w = cg % kPairs == p ? row[p] : w;
-        const int r = r0 + rq * 4 + (cg & 3) + (cg >> 2) * 64;
-        if (r < R)
-          store_scale(out, r, c0 / kTile, c0 + kTile >= C, block_scale_byte<E5M2>(cg >= kPairs ? w >> 16 : w & 0xffffu));
-      }
+      if (WANT & kRows) m[p] = __vmaxu2(__vmaxu2(w[0], w[1]), __vmaxu2(w[2], w[3]));
     }
     if (WANT & kCols) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) col[j] = __vmaxu2(col[j], __shfl_xor_sync(0xffffffffu, col[j], 16));
-      if (lane < 16)
-        *reinterpret_cast<uint4*>(&sm.part[warp][cg * 4]) = make_uint4(col[0], col[1], col[2], col[3]);
-      __syncthreads();
+      if (lane < 16) *reinterpret_cast<uint4*>(&part[warp][cg * 4]) = make_uint4(col[0], col[1], col[2], col[3]);
+    }
+    if (WANT & kRows) {
+      uint32_t mine = 0u;   // lane cg stores the scale of row cg of the thread's
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        const uint4 p = *reinterpret_cast<const uint4*>(&sm.part[k][cg * 4]);
-        col[0] = __vmaxu2(col[0], p.x);
-        col[1] = __vmaxu2(col[1], p.y);
-        col[2] = __vmaxu2(col[2], p.z);
-        col[3] = __vmaxu2(col[3], p.w);
+      for (int p = 0; p < kPairs; ++p) {
+        uint32_t w = __vmaxu2(__byte_perm(m[p], m[p + kPairs], 0x5410), __byte_perm(m[p], m[p + kPairs], 0x7632));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) w = __vmaxu2(w, __shfl_xor_sync(0xffffffffu, w, o));
+        block_inverse2<E5M2>(w, rs[p], rs[p + kPairs]);
+        mine = cg % kPairs == p ? w : mine;
       }
+      const int r = r0 + rq * 4 + (cg & 3) + (cg >> 2) * 64;
+      if (cg < kMine && r < R)
+        store_scale(out, r, c0 / kTile, c0 + kTile >= C,
+                    block_scale_byte<E5M2>(cg >= kPairs ? mine >> 16 : mine & 0xffffu));
+    }
+  }
+
+  // Word `word` of 64: columns 2 word and 2 word + 1.
+  static __device__ __forceinline__ void join_cols(const uint32_t (&part)[16][64], float2 (&cols)[64], int word, int r0,
+                                                   int c0, int R, int C, const BlockOut& out_t) {
+    uint32_t m = 0u;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        cs[j] = f2_of(block_inverse<E5M2>(col[j] & 0xffffu), block_inverse<E5M2>(col[j] >> 16));
-      if (rq < 8 && c < C) {   // thread row rq stores the scale of column rq of the thread's eight
-        const uint32_t w = rq & 4 ? (rq & 2 ? col[3] : col[2]) : (rq & 2 ? col[1] : col[0]);
-        store_scale(out_t, c + rq, r0 / kTile, r0 + kTile >= R, block_scale_byte<E5M2>(rq & 1 ? w >> 16 : w & 0xffffu));
+    for (int k = 0; k < kWarps; ++k) m = __vmaxu2(m, part[k][word]);
+    block_inverse2<E5M2>(m, cols[word].x, cols[word].y);
+    const int c = c0 + 2 * word;
+    if (c < C) {   // (C is even)
+      store_scale(out_t, c, r0 / kTile, r0 + kTile >= R, block_scale_byte<E5M2>(m & 0xffffu));
+      store_scale(out_t, c + 1, r0 / kTile, r0 + kTile >= R, block_scale_byte<E5M2>(m >> 16));
+    }
+  }
+
+  // ONE: every value is multiplied by rs[0].
+  template <int ONE>
+  static __device__ __forceinline__ void write(const uint4 (&v)[U][4], const float (&rs)[kMine], const float2 (&cols)[64],
+                                               uint32_t* tile, int r0, int c0, int R, int C, const BlockOut& out) {
+    const int cg = threadIdx.x & 15, rq = threadIdx.x >> 4, c = c0 + cg * 8;
+    f2 cs[4];
+    if (ONE) {
+      cs[0] = cs[1] = cs[2] = cs[3] = f2_of(rs[0], rs[0]);
+    } else if (WANT & kCols) {
+      const float4 a = *reinterpret_cast<const float4*>(&cols[cg * 4]), b = *reinterpret_cast<const float4*>(&cols[cg * 4 + 2]);
+      cs[0] = f2_of(a.x, a.y);
+      cs[1] = f2_of(a.z, a.w);
+      cs[2] = f2_of(b.x, b.y);
+      cs[3] = f2_of(b.z, b.w);
+    }
+    // Word `rg` (four rows) of a column of group cg lies at rg ^ 2 cg: the words that a warp writes at a time
+    // are in different banks, and four of a column stay together for the 16-byte reads.
+    uint8_t* orow = WANT & kRows ? out.data + (long long)(r0 + rq * 4) * out.ld + c : nullptr;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      uint32_t b[4][2], q[2][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w[4] = {v[u][i].x, v[u][i].y, v[u][i].z, v[u][i].w};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const f2 lo = f2_bf16(w[2 * k]), hi = f2_bf16(w[2 * k + 1]);
+          if (ONE || (WANT & kCols)) {
+            const float2 x = f2_get(f2_mul(lo, cs[2 * k])), y = f2_get(f2_mul(hi, cs[2 * k + 1]));
+            q[k][i] = cast4<E5M2>(x.x, x.y, y.x, y.y);
+          }
+          if (ONE) {
+            b[i][k] = q[k][i];
+          } else if (WANT & kRows) {
+            const f2 s = f2_of(rs[4 * u + i], rs[4 * u + i]);
+            const float2 x = f2_get(f2_mul(lo, s)), y = f2_get(f2_mul(hi, s));
+            b[i][k] = cast4<E5M2>(x.x, x.y, y.x, y.y);
+          }
+        }
+        if (WANT & kRows) {
+          if (r0 + rq * 4 + u * 64 + i < R && c < C)
+            *reinterpret_cast<uint2*>(orow + (u * 64 + i) * out.ld) = make_uint2(b[i][0], b[i][1]);
+        }
+      }
+      if (WANT & kCols) {
+        const int rg = rq + u * 16;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          transpose4(q[k]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) tile[(cg * 8 + k * 4 + j) * 32 + (rg ^ (2 * cg))] = q[k][j];
+        }
       }
     }
   }
 
-  // Word `rg` (four rows) of a column of group cg lies at rg ^ 2 cg: the words that a warp writes at a time
-  // are in different banks, and four of a column stay together for the 16-byte reads.
-  uint8_t* orow = WANT & kRows ? out.data + (long long)(r0 + rq * 4) * out.ld + c : nullptr;
+  // Row c of out_t holds column c of the tile: 16 rows of it a piece.
+  static __device__ __forceinline__ void copy_cols(const uint32_t* tile, int r0, int c0, int C, const BlockOut& out_t) {
+    const int m = threadIdx.x & 7, tc0 = threadIdx.x >> 3;
+    uint8_t* ocol = out_t.data + (long long)(c0 + tc0) * out_t.ld + r0 + m * 16;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    uint32_t b[4][2];
-    uint32_t q[2][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w[4] = {v[u][i].x, v[u][i].y, v[u][i].z, v[u][i].w};
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const f2 lo = f2_bf16(w[2 * k]), hi = f2_bf16(w[2 * k + 1]);
-        if (TILED || (WANT & kCols)) {
-          const float2 x = f2_get(f2_mul(lo, cs[2 * k])), y = f2_get(f2_mul(hi, cs[2 * k + 1]));
-          q[k][i] = cast4<E5M2>(x.x, x.y, y.x, y.y);
-        }
-        if (TILED) {
-          b[i][k] = q[k][i];
-        } else if (WANT & kRows) {
-          const f2 s = f2_of(rs[4 * u + i], rs[4 * u + i]);
-          const float2 x = f2_get(f2_mul(lo, s)), y = f2_get(f2_mul(hi, s));
-          b[i][k] = cast4<E5M2>(x.x, x.y, y.x, y.y);
-        }
-      }
-      if (WANT & kRows) {
-        if (r0 + rq * 4 + u * 64 + i < R && c < C)
-          *reinterpret_cast<uint2*>(orow + (u * 64 + i) * out.ld) = make_uint2(b[i][0], b[i][1]);
-      }
-    }
-    if (WANT & kCols) {
-      const int rg = rq + u * 16;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        transpose4(q[k]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sm.tile[(cg * 8 + k * 4 + j) * 32 + (rg ^ (2 * cg))] = q[k][j];
-      }
+    for (int k = 0; k < 2 * U; ++k) {
+      const int tc = tc0 + k * (64 / U), g = tc >> 3;
+      uint4 w = *reinterpret_cast<const uint4*>(tile + tc * 32 + 4 * (m ^ (g >> 1)));
+      if (g & 1) w = make_uint4(w.z, w.w, w.x, w.y);
+      if (c0 + tc < C && r0 + m * 16 < out_t.ld) *reinterpret_cast<uint4*>(ocol + k * (64 / U) * out_t.ld) = w;
     }
   }
-  if (!(WANT & kCols)) return;
-  __syncthreads();
-  // row c of out_t holds column c of the tile: 16 rows of it a piece
-  const int m = threadIdx.x & 7, tc0 = threadIdx.x >> 3;
-  uint8_t* ocol = out_t.data + (long long)(c0 + tc0) * out_t.ld + r0 + m * 16;
+};
+
+// One tile by itself.
+template <int TILED, int E5M2, int WANT, int U>
+__device__ __forceinline__ void cast_tile(const uint4 (&v)[U][4], CastSmem<1>& sm, int r0, int c0, int R, int C,
+                                          const BlockOut& out, const BlockOut& out_t) {
+  using K = Cast<E5M2, WANT, U>;
+  float rs[K::kMine];
+  if (TILED) {
+    uint32_t m = 0u;
 #pragma unroll
-  for (int k = 0; k < 2 * U; ++k) {
-    const int tc = tc0 + k * (64 / U), g = tc >> 3;
-    uint4 w = *reinterpret_cast<const uint4*>(sm.tile + tc * 32 + 4 * (m ^ (g >> 1)));
-    if (g & 1) w = make_uint4(w.z, w.w, w.x, w.y);
-    if (c0 + tc < C && r0 + m * 16 < out_t.ld) *reinterpret_cast<uint4*>(ocol + k * (64 / U) * out_t.ld) = w;
+    for (int p = 0; p < K::kMine; ++p) {
+      const uint4& q = v[p / 4][p % 4];
+      m = __vmaxu2(m, __vmaxu2(__vmaxu2(q.x & K::kAbs, q.y & K::kAbs), __vmaxu2(q.z & K::kAbs, q.w & K::kAbs)));
+    }
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+    if ((threadIdx.x & 31) == 0) sm.all[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < K::kWarps; ++k) m = max(m, sm.all[k]);
+    rs[0] = block_inverse<E5M2>(m);
+    if (threadIdx.x < kTile) {
+      const uint32_t e = block_scale_byte<E5M2>(m);
+      if ((WANT & kRows) && r0 + threadIdx.x < R) store_scale(out, r0 + threadIdx.x, c0 / kTile, c0 + kTile >= C, e);
+      if ((WANT & kCols) && c0 + threadIdx.x < C) store_scale(out_t, c0 + threadIdx.x, r0 / kTile, r0 + kTile >= R, e);
+    }
+  } else {
+    K::maxima(v, sm.part[0], rs, r0, c0, R, C, out);
+    if (WANT & kCols) {
+      __syncthreads();
+      if (threadIdx.x < 64) K::join_cols(sm.part[0], sm.cols[0], threadIdx.x, r0, c0, R, C, out_t);
+      __syncthreads();
+    }
+  }
+  K::template write<TILED>(v, rs, sm.cols[0], sm.tile[0], r0, c0, R, C, out);
+  if (WANT & kCols) {
+    __syncthreads();
+    K::copy_cols(sm.tile[0], r0, c0, C, out_t);
   }
 }
 
@@ -225,7 +256,7 @@ template <int TILED, int E5M2, int WANT, int SUM>
 __global__ void __launch_bounds__(256, 4)
     block_cast_kernel(const bf16* __restrict__ x, int R, int C, long long ldx, BlockOut out, BlockOut out_t,
                       float* __restrict__ colsum, int tiles_c) {
-  __shared__ __align__(16) CastSmem sm;
+  __shared__ __align__(16) CastSmem<1> sm;
   pdl_wait();
   pdl_trigger();
   const int rt = blockIdx.x / tiles_c;
@@ -243,7 +274,7 @@ __global__ void __launch_bounds__(256, 4)
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[j] = f2_add(s[j], t[j]);
     }
-    float* part = reinterpret_cast<float*>(sm.tile);   // [16 thread rows][128 columns]
+    float* part = reinterpret_cast<float*>(sm.tile[0]);   // [16 thread rows][128 columns]
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 t = f2_get(s[j]);
@@ -272,7 +303,7 @@ template <int KIND>
 __global__ void __launch_bounds__(512)
     block_glu_fwd_kernel(const bf16* __restrict__ gate, const bf16* __restrict__ up, long long ld, int T, int I,
                          BlockOut h, int tiles_c) {
-  __shared__ __align__(16) CastSmem sm;
+  __shared__ __align__(16) CastSmem<1> sm;
   pdl_wait();
   pdl_trigger();
   const int rt = blockIdx.x / tiles_c;
@@ -289,12 +320,16 @@ __global__ void __launch_bounds__(512)
 // [T, 2 I], gate columns first) and of 128 tokens (`d_t` [2 I, T]), and h once more, in blocks of 128 tokens
 // (`h_t` [I, T]): the operands of the input gradient and of both weight gradients from one read. I is a
 // multiple of 128, so that no block holds columns of both. WANT: of the gradients' layouts; H: h.
+constexpr int kGluSmem = sizeof(CastSmem<3>);
 template <int KIND, int WANT, int H>
 __global__ void __launch_bounds__(512, 2)
     block_glu_bwd_kernel(const bf16* __restrict__ dh, long long ld_dh, const bf16* __restrict__ gate,
                          const bf16* __restrict__ up, long long ld, int T, int I, BlockOut d, BlockOut d_t,
                          BlockOut h_t, int tiles_c) {
-  __shared__ __align__(16) CastSmem sm;
+  using K = Cast<0, WANT, 1>;
+  using KH = Cast<0, kCols, 1>;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  CastSmem<3>& sm = *reinterpret_cast<CastSmem<3>*>(smem_raw);
   pdl_wait();
   pdl_trigger();
   const int rt = blockIdx.x / tiles_c;
@@ -305,14 +340,32 @@ __global__ void __launch_bounds__(512, 2)
   load_tile(x, dh, ld_dh, r0, c0, T, I);
 #pragma unroll
   for (int i = 0; i < 4; ++i) block_glu_grad8<KIND>(g[0][i], u[0][i], x[0][i]);
+  float rg[K::kMine], ru[K::kMine], none[K::kMine];
   if (WANT) {
-    cast_tile<0, 0, WANT, 1>(g, sm, r0, c0, T, 2 * I, d, d_t);
-    __syncthreads();
-    cast_tile<0, 0, WANT, 1>(u, sm, r0, I + c0, T, 2 * I, d, d_t);
+    K::maxima(g, sm.part[0], rg, r0, c0, T, 2 * I, d);
+    K::maxima(u, sm.part[1], ru, r0, I + c0, T, 2 * I, d);
   }
-  if (H) {
+  if (H) KH::maxima(x, sm.part[2], none, r0, c0, T, I, BlockOut{});
+  constexpr bool kT = WANT & kCols;
+  if (kT || H) {
     __syncthreads();
-    cast_tile<0, 0, kCols, 1>(x, sm, r0, c0, T, I, BlockOut{}, h_t);
+    const int a = threadIdx.x >> 6, word = threadIdx.x & 63;
+    if (kT && a < 2) K::join_cols(sm.part[a], sm.cols[a], word, r0, a * I + c0, T, 2 * I, d_t);
+    if (H && a == 2) KH::join_cols(sm.part[2], sm.cols[2], word, r0, c0, T, I, h_t);
+    __syncthreads();
+  }
+  if (WANT) {
+    K::template write<0>(g, rg, sm.cols[0], sm.tile[0], r0, c0, T, 2 * I, d);
+    K::template write<0>(u, ru, sm.cols[1], sm.tile[1], r0, I + c0, T, 2 * I, d);
+  }
+  if (H) KH::template write<0>(x, none, sm.cols[2], sm.tile[2], r0, c0, T, I, BlockOut{});
+  if (kT || H) {
+    __syncthreads();
+    if (kT) {
+      K::copy_cols(sm.tile[0], r0, c0, 2 * I, d_t);
+      K::copy_cols(sm.tile[1], r0, I + c0, 2 * I, d_t);
+    }
+    if (H) KH::copy_cols(sm.tile[2], r0, c0, I, h_t);
   }
 }
 
@@ -435,7 +488,14 @@ int block_glu_bwd(int kind, const void* dh, long long ld_dh, const void* gate, c
   LB_GLU(3, 0);
   LB_GLU(3, 1);
 #undef LB_GLU
-  return launch_pdl(kern, dim3(grid), dim3(512), 0, stream, pdl_enabled(11LL * T * I), 1, static_cast<const bf16*>(dh), ld_dh,
+  static bool configured[2][4][2][kMaxDevices] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -10;
+  bool& done = configured[kind == kSwiglu ? 0 : 1][want][h][dev];
+  if (!done && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kGluSmem) != cudaSuccess)
+    return -10;
+  done = true;
+  return launch_pdl(kern, dim3(grid), dim3(512), kGluSmem, stream, pdl_enabled(11LL * T * I), 1, static_cast<const bf16*>(dh), ld_dh,
                     static_cast<const bf16*>(gate), static_cast<const bf16*>(up), ld, T, I, block_out(d),
                     block_out(d_t), block_out(h_t), I / kTile);
 }

@@ -37,6 +37,12 @@ int block_gemm(const BlockPlan& p, const BlockMat& A, const BlockMat& B, void* C
                long long ldc, int out_fp32, int accumulate, const void* bias, void* ws, int* status,
                cudaStream_t stream);
 
+// The product of few rows whose A is bf16 still (rows ldx elements apart) and cast in the kernel, where
+// block_casts_itself says so.
+bool block_casts_itself(const BlockPlan& p, int M, int K);
+int block_gemm_cast(const BlockPlan& p, const void* x, long long ldx, const BlockMat& B, void* C, int M, int N, int K,
+                    long long ldc, int out_fp32, const void* bias, int* status, cudaStream_t stream);
+
 int block_gemm_1cta(int tn, int splits, const BlockMat& A, const BlockMat& B, void* C, int M, int N, int K,
                     long long ldc, int out_fp32, int accumulate, const void* bias, int* status,
                     cudaStream_t stream);

@@ -140,16 +140,18 @@ MlpStorage mlp_storage(int T, int H, int I, int need, void* saved, void* tmp) {
   return s;
 }
 
-// y = (act(x Wgᵀ) * (x Wuᵀ)) Wdᵀ from cast operands; keep_gu: the products stay in s.gu.
-void mlp_products(Call& c, int kind, const MlpStorage& s, int T, int H, int I, bool keep_gu, void* y) {
-  const BlockMat up = rows_of(s.w, I);
-  if (block_glu_fused(T, I, H)) {
+// y = (act(x Wgᵀ) * (x Wuᵀ)) Wdᵀ from cast operands. The two products stay in s.gu for the backward, are dropped, or
+// are there already.
+enum GateUp { kKeepProducts, kDropProducts, kHaveProducts };
+void mlp_products(Call& c, int kind, const MlpStorage& s, int T, int H, int I, GateUp gu, void* y) {
+  const bool keep = gu == kKeepProducts;
+  if (gu != kHaveProducts && block_glu_fused(T, I, H)) {
     c.run([&] {
-      return block_gemm_glu(kind, s.x, s.w, up, T, I, H, keep_gu ? s.gu : nullptr, keep_gu ? s.gu + I : nullptr,
-                            2LL * I, s.h, c.status, c.stream);
+      return block_gemm_glu(kind, s.x, s.w, rows_of(s.w, I), T, I, H, keep ? s.gu : nullptr,
+                            keep ? s.gu + I : nullptr, 2LL * I, s.h, c.status, c.stream);
     });
   } else {
-    c.product(s.x, s.w, Out{s.gu, 0}, T, 2 * I, H, 2LL * I);
+    if (gu != kHaveProducts) c.product(s.x, s.w, Out{s.gu, 0}, T, 2 * I, H, 2LL * I);
     c.run([&] { return block_glu_fwd(kind, s.gu, s.gu + I, 2LL * I, T, I, s.h, c.stream); });
   }
   c.product(s.h, s.wd, Out{y, 0}, T, H, I, H);
@@ -185,6 +187,7 @@ extern "C" int lb_linear_block_fwd(const void* x, long long ldx, const void* w, 
 
 // The same with a weight in 8 bits (bytes, rows ldw apart; scale words, rows_w a group). tmp: lb_linear_kept_bytes.
 extern "C" long long lb_linear_kept_bytes(int T, int K, int N) {
+  if (block_casts_itself(block_plan(T, N, K, !(N & 7)), T, K)) return 0;
   Arena a(nullptr);
   a.mat(T, K);
   a.take(product_bytes(T, N, K));
@@ -194,9 +197,18 @@ extern "C" int lb_linear_kept_fwd(const void* x, long long ldx, const void* w, l
                                   long long rows_w, int w_e5m2, const void* bias, int T, int K, int N, int y_mode,
                                   void* y, void* tmp, int* status, void* stream_) {
   if (T <= 0 || K <= 0 || N <= 0) return -3;
+  const BlockMat wq{(uint8_t*)w, ldw, (uint32_t*)scales, rows_w, w_e5m2};
+  Call c{status, reinterpret_cast<cudaStream_t>(stream_), nullptr};
+  const BlockPlan p = block_plan(T, N, K, !(N & 7));
+  if (block_casts_itself(p, T, K)) {
+    c.run([&] {
+      return block_gemm_cast(p, x, ldx, wq, y, T, N, K, N, y_mode, bias, status, c.stream);
+    });
+    return c.rc;
+  }
   Arena a(tmp);
-  const BlockMat xq = a.mat(T, K), wq{(uint8_t*)w, ldw, (uint32_t*)scales, rows_w, w_e5m2};
-  Call c{status, reinterpret_cast<cudaStream_t>(stream_), a.take(0)};
+  const BlockMat xq = a.mat(T, K);
+  c.ws = a.take(0);
   c.run([&] { return block_cast(x, T, K, ldx, 0, 0, xq, BlockMat{}, 0, nullptr, c.stream); });
   c.product(xq, wq, Out{y, y_mode}, T, N, K, N, bias);
   return c.rc;
@@ -245,16 +257,20 @@ extern "C" int lb_mlp_block_fwd(int kind, const void* x, long long ldx, const vo
     c.run([&] { return block_cast(wu, I, H, ldu, 1, 0, rows_of(s.w, I), t, I / kScaleBlock, nullptr, c.stream); });
   }
   c.run([&] { return block_cast(wd, H, I, ldd, 1, 0, s.wd, s.wd_t, 0, nullptr, c.stream); });
-  mlp_products(c, kind, s, T, H, I, true, y);
+  mlp_products(c, kind, s, T, H, I, kKeepProducts, y);
   return c.rc;
 }
 
 // The same with weights in 8 bits, gate and up fused. tmp: lb_mlp_kept_bytes.
 namespace {
-MlpStorage mlp_kept_storage(int T, int H, int I, void* tmp) {
+// Whether the gate and up product casts x itself.
+bool mlp_casts_itself(int T, int H, int I, const BlockPlan& p) {
+  return !block_glu_fused(T, I, H) && block_casts_itself(p, T, H);
+}
+MlpStorage mlp_kept_storage(int T, int H, int I, bool cast_x, void* tmp) {
   MlpStorage s{};
   Arena a(tmp);
-  s.x = a.mat(T, H);
+  if (!cast_x) s.x = a.mat(T, H);
   s.h = a.mat(T, I);
   if (!block_glu_fused(T, I, H)) s.gu = static_cast<__nv_bfloat16*>(a.take(size_t(T) * 2 * I * 2));
   s.ws_fwd = a.take(max2(product_bytes(T, 2 * I, H), product_bytes(T, H, I)));
@@ -263,19 +279,25 @@ MlpStorage mlp_kept_storage(int T, int H, int I, void* tmp) {
 }
 }  // namespace
 extern "C" long long lb_mlp_kept_bytes(int T, int H, int I) {
-  return (long long)mlp_kept_storage(T, H, I, nullptr).fwd;
+  const bool cast_x = mlp_casts_itself(T, H, I, block_plan(T, 2 * I, H, true));
+  return (long long)mlp_kept_storage(T, H, I, cast_x, nullptr).fwd;
 }
 extern "C" int lb_mlp_kept_fwd(int kind, const void* x, long long ldx, const void* w, long long ldw, const void* ws,
                                long long rows_w, int w_e5m2, const void* wd, long long ldd, const void* wds,
                                long long rows_d, int wd_e5m2, int T, int H, int I, void* y, void* tmp, int* status,
                                void* stream_) {
   if (T <= 0 || H <= 0 || I <= 0 || (I % kScaleBlock)) return -3;
-  MlpStorage s = mlp_kept_storage(T, H, I, tmp);
+  const BlockPlan p = block_plan(T, 2 * I, H, true);
+  const bool cast_x = mlp_casts_itself(T, H, I, p);
+  MlpStorage s = mlp_kept_storage(T, H, I, cast_x, tmp);
   s.w = BlockMat{(uint8_t*)w, ldw, (uint32_t*)ws, rows_w, w_e5m2};
   s.wd = BlockMat{(uint8_t*)wd, ldd, (uint32_t*)wds, rows_d, wd_e5m2};
   Call c{status, reinterpret_cast<cudaStream_t>(stream_), s.ws_fwd};
-  c.run([&] { return block_cast(x, T, H, ldx, 0, 0, s.x, BlockMat{}, 0, nullptr, c.stream); });
-  mlp_products(c, kind, s, T, H, I, false, y);
+  if (cast_x)
+    c.run([&] { return block_gemm_cast(p, x, ldx, s.w, s.gu, T, 2 * I, H, 2LL * I, 0, nullptr, status, c.stream); });
+  else
+    c.run([&] { return block_cast(x, T, H, ldx, 0, 0, s.x, BlockMat{}, 0, nullptr, c.stream); });
+  mlp_products(c, kind, s, T, H, I, cast_x ? kHaveProducts : kDropProducts, y);
   return c.rc;
 }
 

@@ -34,6 +34,19 @@ __device__ __forceinline__ float block_inverse(uint32_t a) {
   const int x = min((E5M2 ? 269 : 262) - int((a + 31u) >> 7), 253);
   return __uint_as_float(a >= 0x7f80u ? 0x7fffffffu : uint32_t(x) << 23);
 }
+// The same for the two halves of a word: with n = 262 (269), 2^(127 - e) has the bits (n - x) << 23, and x << 23 is
+// (a + 31) & 0xff80, 16 bits up.
+template <int E5M2>
+__device__ __forceinline__ void block_inverse2(uint32_t w, float& lo, float& hi) {
+  constexpr uint32_t kTop = (E5M2 ? 269u : 262u) << 23, kMost = 253u << 23;
+  const uint32_t x = (w + 0x001f001fu) & 0xff80ff80u;
+  lo = __uint_as_float(min(kTop - (x << 16), kMost));
+  hi = __uint_as_float(min(kTop - (x & 0xffff0000u), kMost));
+  if (((w & 0xffffu) >= 0x7f80u) || w >= 0x7f800000u) {   // hardly ever
+    lo = (w & 0xffffu) >= 0x7f80u ? __uint_as_float(0x7fffffffu) : lo;
+    hi = w >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : hi;
+  }
+}
 // The scale byte that goes with it.
 template <int E5M2>
 __device__ __forceinline__ uint32_t block_scale_byte(uint32_t a) {
@@ -89,6 +102,12 @@ __device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t
       :
       : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
       : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x4(uint32_t taddr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(a), "r"(b), "r"(c),
+               "r"(d)
+               : "memory");
 }
 
 }  // namespace lb

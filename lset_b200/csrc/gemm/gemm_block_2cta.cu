@@ -75,12 +75,6 @@ __device__ __forceinline__ void umma2_block(uint32_t tmem_d, uint64_t adesc, uin
       : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x4(uint32_t taddr, const uint32_t (&r)[4]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3])
-               : "memory");
-}
-
 template <typename OutT, int GLU>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_block_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -274,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         const uint32_t dst = tmem_base + lanes + kScaleCols + 16 * slot;
-        tmem_st_32x32b_x4(dst, wa);
+        tmem_st_32x32b_x4(dst, wa[0], wa[1], wa[2], wa[3]);
         tmem_st_32x32b_x8(dst + 4, wb);
         tmem_st_wait();
         tc_fence_before();
@@ -297,12 +291,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t over = map_to_cta(tover, 0);
     uint8_t* sblk = reinterpret_cast<uint8_t*>(epi_stage + (warp - 2) * EPI_WORDS);
     int it = 0;
+    bool ok = true;
     for (int tile = pair; tile < total; tile += npairs, ++it) {
       decode(tile, split, m0, n0, st0, st1);
       const int acc = it & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (it >> 1) & 1))) {
+      if (ok && !__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (it >> 1) & 1))) {
         report_status(g.status, kStatusTimeoutEpilogue);
-        break;
+        ok = false;
+      }
+      if (!ok) {   // (the two warps of a row meet at a barrier for each tile, whatever either has waited for)
+        if (GLU) asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+        continue;
       }
       tc_fence_after();
       const uint32_t src0 = tmem_base + (uint32_t(q * 32) << 16) + (acc ? kAcc1 : 0);

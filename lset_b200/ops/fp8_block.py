@@ -466,10 +466,11 @@ def linear_fp8_block(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) ->
         if bias is not None:
             bias = bias.to(torch.bfloat16).contiguous()
         y = torch.empty((T, N), dtype=act, device=x.device)
-        tmp = _bytes(_linear_kept_bytes(T, K, N), x.device)
+        n = _linear_kept_bytes(T, K, N)
+        tmp = _bytes(n, x.device) if n else None      # none: the product casts x itself
         _call("lb_linear_kept_fwd", x2.data_ptr(), x2.stride(0), *w._where, w._e5m2, nv.ptr(bias), T, K, N, fp32,
-              y.data_ptr(), tmp.data_ptr(), _status_ptr(x.device), nv.stream_ptr())
-        nv.count_launch(2)
+              y.data_ptr(), nv.ptr(tmp), _status_ptr(x.device), nv.stream_ptr())
+        nv.count_launch(2 if n else 1)
     return y if x2.dim() == x.dim() else y.view(*x.shape[:-1], N)
 
 

@@ -172,11 +172,11 @@ def _off(a, b):
     return float((a.double() - b).norm() / b.norm().clamp(min=1e-300))
 
 
-TOKENS = [1, 2, 15, 64, 129, 333, 1000, 2600]
+TOKENS = [1, 2, 15, 16, 17, 31, 32, 33, 64, 129, 333, 1000, 2600]
 
 
 @pytest.mark.parametrize("T", TOKENS)
-@pytest.mark.parametrize("K,N,bias", [(136, 264, True), (1024, 512, False), (640, 72, True)])
+@pytest.mark.parametrize("K,N,bias", [(136, 264, True), (1024, 512, False), (640, 72, True), (4104, 256, False)])
 def test_linear_forward_and_gradients(T, K, N, bias):
     x, w, dy = _rand(T, K, spread=1.0), _rand(N, K, seed=1, spread=0.5), _rand(T, N, seed=2, spread=1.0)
     b = _rand(N, seed=3, spread=0.5) if bias else None
