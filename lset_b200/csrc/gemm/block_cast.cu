@@ -32,13 +32,14 @@ __device__ __forceinline__ void transpose4(uint32_t (&w)[4]) {
 
 // One 8-bit matrix to write: bytes ld apart, scale words as block_scale.cuh lays them out (`rows` words a
 // group of four blocks). kb0: block of a row that the first byte belongs to, where only part of the
-// columns is written.
+// columns is written; fill: the last block written is the row's last, and the rest of its word is filled.
 struct BlockOut {
   uint8_t* data;
   long long ld;
   uint32_t* scales;
   long long rows;
   int kb0;
+  bool fill;
 };
 
 // Scale byte e of block kb of row r; with the last block of a row, the rest of its word.
@@ -46,7 +47,7 @@ __device__ __forceinline__ void store_scale(const BlockOut& o, long long r, int 
   kb += o.kb0;
   uint8_t* p = reinterpret_cast<uint8_t*>(o.scales + (kb >> 2) * o.rows + r);
   p[kb & 3] = uint8_t(e);
-  if (last)
+  if (last && o.fill)
     for (int k = (kb & 3) + 1; k < 4; ++k) p[k] = uint8_t(kScaleOne);
 }
 
@@ -298,6 +299,39 @@ __global__ void __launch_bounds__(256, 4)
   if (WANT) cast_tile<TILED, E5M2, WANT, 2>(v, sm, r0, c0, R, C, out, out_t);
 }
 
+// Several casts in one launch, both layouts of each: the activations and the weights of a layer, which do not wait for one
+// another. Measured for x [257, 1024] and w [2048, 1024]: 3.9 + 3.3 us in launches of their own, with 1.6 between them;
+// x [4097, 2048], w [16384, 2048] and [2048, 8192]: see the training step's table.
+struct CastJob {
+  const bf16* x;
+  int R, C;
+  long long ldx;
+  int tiled, tiles_c;
+  unsigned first;   // its first CTA
+  BlockOut out, out_t;
+};
+struct CastJobs {
+  CastJob job[kMaxCasts];
+};
+__global__ void __launch_bounds__(256, 4) block_casts_kernel(const __grid_constant__ CastJobs jobs) {
+  __shared__ __align__(16) CastSmem<1> sm;
+  pdl_wait();
+  pdl_trigger();
+  int j = 0;
+#pragma unroll
+  for (int k = 1; k < kMaxCasts; ++k)
+    if (blockIdx.x >= jobs.job[k].first) j = k;
+  const CastJob& g = jobs.job[j];
+  const int at = int(blockIdx.x - g.first), rt = at / g.tiles_c;
+  const int r0 = rt * kTile, c0 = (at - rt * g.tiles_c) * kTile;
+  uint4 v[2][4];
+  load_tile(v, g.x, g.ldx, r0, c0, g.R, g.C);
+  if (g.tiled)
+    cast_tile<1, 0, kRows | kCols, 2>(v, sm, r0, c0, g.R, g.C, g.out, g.out_t);
+  else
+    cast_tile<0, 0, kRows | kCols, 2>(v, sm, r0, c0, g.R, g.C, g.out, g.out_t);
+}
+
 // h = act(gate) * up of [T, I] matrices (rows ld elements apart), rounded to bf16, in blocks of a row.
 template <int KIND>
 __global__ void __launch_bounds__(512)
@@ -401,7 +435,9 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-BlockOut block_out(const BlockMat& m, int kb0 = 0) { return BlockOut{m.data, m.ld, m.scales, m.rows_s, kb0}; }
+BlockOut block_out(const BlockMat& m, int kb0 = 0, bool fill = true) {
+  return BlockOut{m.data, m.ld, m.scales, m.rows_s, kb0, fill};
+}
 
 // CTAs of the tiles of [R, C]; 0 where there are too many.
 unsigned cast_grid(int R, int C) {
@@ -450,6 +486,36 @@ int block_cast(const void* x, int R, int C, long long ldx, int tiled, int e5m2, 
   return launch_pdl(kern, dim3(grid), dim3(256), 0, stream, pdl_enabled(4LL * R * C), 1,
                     static_cast<const bf16*>(x), R, C, ldx, block_out(out), block_out(out_t, kb0_t), colsum,
                     (C + kTile - 1) / kTile);
+}
+
+int block_casts(const BlockCast* jobs, int n, cudaStream_t stream) {
+  if (n < 1 || n > kMaxCasts) return -3;
+  CastJobs all{};
+  long long tiles = 0, bytes = 0;
+  bool both = n > 1;
+  for (int i = 0; i < n; ++i) both = both && jobs[i].out.data != nullptr && jobs[i].out_t.data != nullptr;
+  if (!both) {   // a layout that is not wanted: launches of their own
+    for (int i = 0; i < n; ++i) {
+      const BlockCast& j = jobs[i];
+      PdlScope scope(i > 0 || pdl_enabled());
+      // (one after the other: a part that fills a word of scales too far is followed by the part that has it)
+      if (const int rc = block_cast(j.x, j.R, j.C, j.ldx, j.tiled, 0, j.out, j.out_t, j.kb0_t, nullptr, stream)) return rc;
+    }
+    return 0;
+  }
+  for (int i = 0; i < kMaxCasts; ++i) {
+    all.job[i].first = 0xffffffffu;
+    if (i >= n) continue;
+    const BlockCast& j = jobs[i];
+    if (j.R <= 0 || j.C <= 0 || (j.C & 7) || (j.ldx & 7) || (reinterpret_cast<uintptr_t>(j.x) & 15)) return -3;
+    if (!fits(j.out, j.R, j.C) || !fits(j.out_t, j.C, j.R) || j.kb0_t < 0 || (j.kb0_t > 0 && (j.R % kTile))) return -3;
+    all.job[i] = CastJob{static_cast<const bf16*>(j.x), j.R, j.C, j.ldx, j.tiled, (j.C + kTile - 1) / kTile,
+                         unsigned(tiles), block_out(j.out), block_out(j.out_t, j.kb0_t, j.fill_t)};
+    tiles += 1LL * all.job[i].tiles_c * ((j.R + kTile - 1) / kTile);
+    bytes += 4LL * j.R * j.C;
+    if (tiles > 0x7fffffffLL) return -3;
+  }
+  return launch_pdl(block_casts_kernel, dim3(unsigned(tiles)), dim3(256), 0, stream, pdl_enabled(bytes), 1, all);
 }
 
 // h = act(gate) * up of [T, I] (rows ld elements apart; I a multiple of 128) in blocks of a row. kind: 0 = SwiGLU,

@@ -59,6 +59,18 @@ int block_gemm_glu(int kind, const BlockMat& A, const BlockMat& Wg, const BlockM
 // [ceil(R / 128)][C], the column sums of each 128 rows of x (null: not wanted).
 int block_cast(const void* x, int R, int C, long long ldx, int tiled, int e5m2, const BlockMat& out,
                const BlockMat& out_t, int kb0_t, float* colsum, cudaStream_t stream);
+// Up to kMaxCasts casts to e4m3 in one launch (where both layouts of all are wanted).
+enum { kMaxCasts = 4 };
+struct BlockCast {
+  const void* x;
+  int R, C;
+  long long ldx;
+  int tiled;
+  BlockMat out, out_t;
+  int kb0_t;
+  bool fill_t;   // out_t's columns end here (not where another cast of the same launch writes on)
+};
+int block_casts(const BlockCast* jobs, int n, cudaStream_t stream);
 int block_glu_fwd(int kind, const void* gate, const void* up, long long ld, int T, int I, const BlockMat& out,
                   cudaStream_t stream);
 int block_glu_bwd(int kind, const void* dh, long long ld_dh, const void* gate, const void* up, long long ld,

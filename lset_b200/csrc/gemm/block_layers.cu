@@ -179,8 +179,8 @@ extern "C" int lb_linear_block_fwd(const void* x, long long ldx, const void* w, 
   if (T <= 0 || K <= 0 || N <= 0) return -3;
   const LinearStorage s = linear_storage(T, K, N, need, saved, tmp);
   Call c{status, reinterpret_cast<cudaStream_t>(stream_), s.ws_fwd};
-  c.run([&] { return block_cast(x, T, K, ldx, 0, 0, s.x, s.x_t, 0, nullptr, c.stream); });
-  c.run([&] { return block_cast(w, N, K, ldw, 1, 0, s.w, s.w_t, 0, nullptr, c.stream); });
+  const BlockCast casts[2] = {{x, T, K, ldx, 0, s.x, s.x_t, 0, true}, {w, N, K, ldw, 1, s.w, s.w_t, 0, true}};
+  c.run([&] { return block_casts(casts, 2, c.stream); });
   c.product(s.x, s.w, Out{y, y_mode}, T, N, K, N, bias);
   return c.rc;
 }
@@ -247,16 +247,16 @@ extern "C" int lb_mlp_block_fwd(int kind, const void* x, long long ldx, const vo
   if (T <= 0 || H <= 0 || I <= 0 || (I % kScaleBlock)) return -3;
   const MlpStorage s = mlp_storage(T, H, I, need, saved, tmp);
   Call c{status, reinterpret_cast<cudaStream_t>(stream_), s.ws_fwd};
-  c.run([&] { return block_cast(x, T, H, ldx, 0, 0, s.x, s.x_t, 0, nullptr, c.stream); });
+  BlockCast casts[4] = {{x, T, H, ldx, 0, s.x, s.x_t, 0, true}, {wd, H, I, ldd, 1, s.wd, s.wd_t, 0, true}};
   if (wu == nullptr) {
-    c.run([&] { return block_cast(wg, 2 * I, H, ldg, 1, 0, s.w, s.w_t, 0, nullptr, c.stream); });
+    casts[2] = BlockCast{wg, 2 * I, H, ldg, 1, s.w, s.w_t, 0, true};
   } else {
-    c.run([&] { return block_cast(wg, I, H, ldg, 1, 0, s.w, s.w_t, 0, nullptr, c.stream); });
     BlockMat t = s.w_t;
     if (t.data != nullptr) t.data += I;   // columns I on: blocks I / 128 on
-    c.run([&] { return block_cast(wu, I, H, ldu, 1, 0, rows_of(s.w, I), t, I / kScaleBlock, nullptr, c.stream); });
+    casts[2] = BlockCast{wg, I, H, ldg, 1, s.w, s.w_t, 0, false};
+    casts[3] = BlockCast{wu, I, H, ldu, 1, rows_of(s.w, I), t, I / kScaleBlock, true};
   }
-  c.run([&] { return block_cast(wd, H, I, ldd, 1, 0, s.wd, s.wd_t, 0, nullptr, c.stream); });
+  c.run([&] { return block_casts(casts, wu == nullptr ? 3 : 4, c.stream); });
   mlp_products(c, kind, s, T, H, I, kKeepProducts, y);
   return c.rc;
 }

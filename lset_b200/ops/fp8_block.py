@@ -340,6 +340,15 @@ def _returned(w, out):
     return None
 
 
+def _storage(n_saved, n_tmp, device):
+    """A tensor of ``n_saved`` bytes for the backward, a tensor to hold during the call (or None), and the address of
+    ``n_tmp`` bytes: behind the first where they are few (an allocation costs the host 2 us), else in the second."""
+    small = n_tmp <= 1 << 20
+    saved = _bytes(n_saved + n_tmp if small else n_saved, device)
+    tmp = None if small else _bytes(n_tmp, device)
+    return saved, tmp, saved.data_ptr() + n_saved if small else tmp.data_ptr()
+
+
 @functools.lru_cache(maxsize=4096)
 def _linear_bytes(T, K, N, need):
     out = (_L * 3)()
@@ -383,12 +392,12 @@ class _LinearFp8Block(torch.autograd.Function):
             if bias is not None:
                 bias = bias.to(torch.bfloat16).contiguous()
             n_saved, n_tmp, _ = _linear_bytes(T, K, N, need)
-            saved, tmp = _bytes(n_saved, x.device), _bytes(n_tmp, x.device)
+            saved, tmp, at = _storage(n_saved, n_tmp, x.device)
             y = torch.empty(*x.shape[:-1], N, dtype=act, device=x.device)
             _call("lb_linear_block_fwd", x2.data_ptr(), x2.stride(0), w2.data_ptr(), w2.stride(0), nv.ptr(bias), T, K, N,
-                  need, _mode(act), y.data_ptr(), saved.data_ptr(), tmp.data_ptr(),
+                  need, _mode(act), y.data_ptr(), saved.data_ptr(), at,
                   _status_ptr(x.device), nv.stream_ptr())
-            nv.count_launch(3)
+            nv.count_launch(2)
         ctx.save_for_backward(w, saved)
         return y
 
@@ -534,12 +543,12 @@ class _GatedMlpFp8Block(torch.autograd.Function):
             x2, wg, wd = _aligned(x2), _aligned(w_gate), _aligned(w_down)
             wu = None if w_up is None else _aligned(w_up)
             n_saved, n_tmp, _ = _mlp_bytes(T, H, I, need)
-            saved, tmp = _bytes(n_saved, x.device), _bytes(n_tmp, x.device)
+            saved, tmp, at = _storage(n_saved, n_tmp, x.device)
             y = torch.empty(x.shape, dtype=torch.bfloat16, device=x.device)
             _call("lb_mlp_block_fwd", _KINDS[kind], x2.data_ptr(), x2.stride(0), wg.data_ptr(), wg.stride(0), nv.ptr(wu),
                   0 if wu is None else wu.stride(0), wd.data_ptr(), wd.stride(0), T, H, I, need, y.data_ptr(),
-                  saved.data_ptr(), tmp.data_ptr(), _status_ptr(x.device), nv.stream_ptr())
-            nv.count_launch(5 + (wu is not None))
+                  saved.data_ptr(), at, _status_ptr(x.device), nv.stream_ptr())
+            nv.count_launch(3)
         ctx.save_for_backward(w_gate, w_up, w_down, saved)
         return y.to(act)
 
