@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(256, 4)
 
 // Several casts in one launch, both layouts of each: the activations and the weights of a layer, which do not wait for one
 // another. Measured for x [257, 1024] and w [2048, 1024]: 3.9 + 3.3 us in launches of their own, with 1.6 between them;
-// x [4097, 2048], w [16384, 2048] and [2048, 8192]: see the training step's table.
+// x [4097, 2048] with w [16384, 2048] and [2048, 8192]: 11.0 + 26.9 + 20.0 us, 38 together.
 struct CastJob {
   const bf16* x;
   int R, C;

@@ -565,7 +565,7 @@ int block_gemm_2cta(int splits, long long split_stride, const BlockMat& A, const
   g.band = band_of(tiles_n, 1LL * N * K);
   g.status = status;
   const long long total = 1LL * tiles_m * tiles_n * splits;
-  if (total > 0x7fffffffLL) return -3;
+  if (total > 0x7fff0000LL) return -3;   // (tiles are counted in steps of the grid)
   return out_fp32 ? launch_2cta<float, 0>(tmA, tmB, tmB, g, total, stream)
                   : launch_2cta<__nv_bfloat16, 0>(tmA, tmB, tmB, g, total, stream);
 }
@@ -606,7 +606,7 @@ int block_gemm_glu(int kind, const BlockMat& A, const BlockMat& Wg, const BlockM
   g.rows_h = h.rows_s;
   g.status = status;
   const long long total = 1LL * tiles_m * tiles_n;
-  if (total > 0x7fffffffLL) return -3;
+  if (total > 0x7fff0000LL) return -3;   // (tiles are counted in steps of the grid)
   return kind == kSwiglu ? launch_2cta<__nv_bfloat16, 1 + kSwiglu>(tmA, tmG, tmU, g, total, stream)
                          : launch_2cta<__nv_bfloat16, 1 + kGeglu>(tmA, tmG, tmU, g, total, stream);
 }

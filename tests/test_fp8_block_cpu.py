@@ -349,3 +349,69 @@ def test_layers_of_biased_models_keep_their_bias():
         assert torch.equal(m[0](x), want) and torch.equal(m(x), last)
     with pytest.raises(ValueError, match="without gradients"):
         m[0](x.requires_grad_())
+
+
+@pytest.mark.parametrize("family", ["qwen3", "llama", "embeddinggemma", "bert"])
+def test_every_family_encodes_with_kept_weights(family):
+    from lset_b200.models import BertConfig, GemmaConfig, LlamaConfig, get_model_spec
+    from lset_b200.models import Qwen3Config
+    from lset_b200.train.quantization.fp8 import Fp8KeptLinear, apply_fp8_inference
+
+    dims = dict(vocab_size=97, hidden_size=64, intermediate_size=128, num_hidden_layers=2, num_attention_heads=4)
+    cfg = {"qwen3": lambda: Qwen3Config(**dims, num_key_value_heads=2, head_dim=16),
+           "llama": lambda: LlamaConfig(**dims, num_key_value_heads=2, head_dim=16),
+           "embeddinggemma": lambda: GemmaConfig(**dims, num_key_value_heads=1, head_dim=16),
+           "bert": lambda: BertConfig(**dims)}[family]()
+    torch.manual_seed(14)
+    model = get_model_spec(family).model_cls(cfg).eval()
+    ids, mask = torch.randint(0, 97, (2, 11)), torch.ones(2, 11, dtype=torch.long)
+    mask[1, 7:] = 0
+    with torch.no_grad():
+        want = model(ids, mask)["hidden_states"]
+        apply_fp8_inference(model)
+        got = model(ids, mask)["hidden_states"]
+    assert sum(isinstance(m, Fp8KeptLinear) for m in model.modules()) == 12
+    keep = mask.bool()
+    assert float(torch.nn.functional.cosine_similarity(got[keep], want[keep], dim=-1).min()) > 0.97
+
+
+def test_gradients_of_some_inputs_of_a_linear_layer():
+    g = torch.Generator().manual_seed(6)
+    mk = lambda *s: torch.randn(*s, generator=g).to(torch.bfloat16)  # noqa: E731
+    x, w, b, dy = mk(2, 9, 64), mk(32, 64), mk(32), mk(2, 9, 32)
+    leaves = [x, w, b]
+    for t in leaves:
+        t.requires_grad_()
+    full = torch.autograd.grad(fb.linear_fp8_block(*leaves), leaves, dy)
+    for i in range(3):
+        for t in leaves:
+            t.requires_grad_(t is leaves[i])
+        (one,) = torch.autograd.grad(fb.linear_fp8_block(*leaves), (leaves[i],), dy)
+        assert one.shape == leaves[i].shape and torch.equal(one, full[i])
+
+
+def test_no_gradient_of_a_gradient():
+    x, w = torch.randn(4, 64, requires_grad=True), torch.randn(32, 64, requires_grad=True)
+    (dx,) = torch.autograd.grad(fb.linear_fp8_block(x, w).sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
+
+
+def test_evaluation_of_a_model_with_the_recipe_keeps_8_bit_weights(monkeypatch):
+    import sys
+    import types
+
+    from lset_b200.config import LSETConfig
+    from lset_b200.eval import mteb_evaluator
+    from lset_b200.eval.run import run_eval
+
+    seen = []
+    monkeypatch.setitem(sys.modules, "mteb", types.SimpleNamespace(
+        get_tasks=lambda tasks: list(tasks), evaluate=lambda *a, **k: types.SimpleNamespace(task_results=[])))
+    monkeypatch.setattr(mteb_evaluator.LSETMTEBModel, "from_pretrained",
+                        classmethod(lambda cls, path, **kw: seen.append(kw.get("fp8", False))))
+    for enabled, recipe in ((True, "block128"), (True, "tensorwise"), (False, "block128")):
+        cfg = LSETConfig()
+        cfg.fp8.enabled, cfg.fp8.recipe = enabled, recipe
+        run_eval(cfg)
+    assert seen == [True, False, False]

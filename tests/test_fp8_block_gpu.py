@@ -283,6 +283,69 @@ def test_gated_mlp_forward_and_gradients(T, H, I, kind):
 # ------------------------------------------------------------------------------------------------
 # Ways of calling
 # ------------------------------------------------------------------------------------------------
+def test_gradients_of_some_inputs_only():
+    x, w, b, dy = _rand(300, 256, spread=1.0), _rand(520, 256, seed=1, spread=0.5), _rand(520, seed=2), _rand(300, 520, seed=3)
+    wg, wu, wd, dz = (_rand(256, 256, seed=4, spread=0.3) * 0.06, _rand(256, 256, seed=5, spread=0.3) * 0.06,
+                      _rand(256, 256, seed=6, spread=0.3) * 0.06, _rand(300, 256, seed=7))
+    for fn, leaves, grad in ((fb.linear_fp8_block, [x, w, b], dy), (fb.gated_mlp_fp8_block, [x, wg, wu, wd], dz)):
+        for t in leaves:
+            t.requires_grad_()
+        full = torch.autograd.grad(fn(*leaves), leaves, grad)
+        for some in range(1, 1 << len(leaves)):
+            for i, t in enumerate(leaves):
+                t.requires_grad_(bool(some >> i & 1))
+            wanted = [t for t in leaves if t.requires_grad]
+            got = torch.autograd.grad(fn(*leaves), wanted, grad)
+            for t, g in zip(wanted, got):
+                want = full[[a is t for a in leaves].index(True)]
+                assert torch.equal(g, want), some
+    nv.check_status()
+
+
+def test_kept_weights_in_the_wider_format_and_as_parts():
+    x = _rand(50, 512, spread=0.5)
+    w, wd = _rand(512, 512, seed=1, spread=0.3) * 0.05, _rand(512, 256, seed=2, spread=0.3) * 0.05
+    with torch.no_grad():
+        for T in (7, 50):
+            for e5m2 in (False, True):
+                q, _ = fb.quantize_fp8_block(w, tile=True, e5m2=e5m2)
+                d, _ = fb.quantize_fp8_block(wd, tile=True, e5m2=e5m2)
+                xq, _ = fb.quantize_fp8_block(x[:T])
+                want = xq.dequantize().double() @ q.dequantize().double().t()
+                assert _off(fb.linear_fp8_block(x[:T], q), want) < 2.0 ** -8
+                part = fb.Fp8BlockTensor(q.data[128:392], 512, q.scales[:, 128:392], e5m2)
+                assert _off(fb.linear_fp8_block(x[:T], part), want[:, 128:392]) < 2.0 ** -8
+                gu = want.to(torch.bfloat16).double()
+                h = (torch.nn.functional.silu(gu[:, :256]) * gu[:, 256:]).to(torch.bfloat16)
+                y = fb.gated_mlp_fp8_block(x[:T], q, None, d)
+                assert _off(y, _value(h, 1, 128) @ d.dequantize().double().t()) < 2.0 ** -7
+    nv.check_status()
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 136, 272), (300, 264, 640), (1500, 2056, 640)])
+def test_outputs_that_start_anywhere(M, N, K):
+    a, _ = fb.quantize_fp8_block(_rand(M, K))
+    b, _ = fb.quantize_fp8_block(_rand(N, K, seed=1), tile=True)
+    for dt in (torch.bfloat16, torch.float32):
+        wide = torch.full((M, N + 9), 7.0, dtype=dt, device="cuda")
+        out = wide[:, 1:N + 1]
+        fb.matmul_fp8_block(a, b, out=out)
+        _check_product(out, a, b)
+        assert (wide[:, 0] == 7).all() and (wide[:, N + 1:] == 7).all()
+
+
+def test_gradients_that_are_no_plain_matrices():
+    x, w = _rand(130, 256, spread=0.5).requires_grad_(), _rand(136, 256, seed=1, spread=0.3).requires_grad_()
+    y = fb.linear_fp8_block(x, w)
+    dy = _rand(136, 130, seed=2)
+    got = torch.autograd.grad(y, (x, w), dy.t(), retain_graph=True)            # transposed
+    want = torch.autograd.grad(y, (x, w), dy.t().contiguous(), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    got = torch.autograd.grad(y.sum(), (x, w), retain_graph=True)              # one value, expanded
+    want = torch.autograd.grad(y, (x, w), torch.ones_like(y))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_no_result_depends_on_timing():
     x, w = _rand(3000, 1040, spread=1.0).requires_grad_(), _rand(520, 1040, seed=1, spread=0.5).requires_grad_()
     b, dy = _rand(520, seed=2, spread=0.5).requires_grad_(), _rand(3000, 520, seed=3, spread=1.0)
