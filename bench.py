@@ -423,7 +423,8 @@ def run_ours(args):
                             "native_library": str(nv.lib_path().name)}, preset)
         if args.fp8 is not None:
             # a side measurement, not the headline: linear layers on the 8-bit tensor-core GEMM
-            line["dtype"] = f"fp8 ({args.fp8}: e4m3 operands, e5m2 gradients) in linear layers, bf16 elsewhere"
+            grads = "e4m3" if args.fp8 == "block128" else "e5m2"
+            line["dtype"] = f"fp8 ({args.fp8}: e4m3 operands, {grads} gradients) in linear layers, bf16 elsewhere"
             line["vs_baseline"] = None
         print(json.dumps(line))
     import torch.distributed as dist
@@ -617,7 +618,8 @@ def main():
     ap.add_argument("--warmup", type=int, default=3)
     ap.add_argument("--impl", choices=["ours", "reference"], default="ours")
     ap.add_argument("--config", choices=sorted(PRESETS), default="qwen3-0.6b")
-    ap.add_argument("--fp8", choices=["tensorwise", "rowwise", "rowwise_with_gw_hp"], default=None,
+    ap.add_argument("--fp8", choices=["tensorwise", "rowwise", "rowwise_with_gw_hp", "block128"],
+                    default=None,
                     help="side measurement: FP8 linear layers (the headline number is bf16)")
     ap.add_argument("--reshard-after-forward", action="store_true",
                     help="side measurement: shard the layers' parameters and gradients as well "
