@@ -323,20 +323,22 @@ def _gradient_of(w):
     """``(tensor, mode)`` that a native call writes the gradient of weight ``w`` to: its fp32 accumulator where the
     sharding runtime has given it one, else a tensor of its type (fp32 for types other than bf16)."""
     main = main_grad_of(w)
-    if main is not None and main.dtype == torch.float32 and main.is_contiguous():
-        return main, _ADD
-    out = torch.empty(w.shape, dtype=torch.bfloat16 if w.dtype == torch.bfloat16 and main is None else torch.float32,
-                      device=w.device)
-    return out, _mode(out.dtype)
-
-
-def _returned(w, out):
-    """What autograd gets for ``w`` once ``_gradient_of``'s tensor is written."""
-    main = main_grad_of(w)
     if main is None:
-        return out.to(w.dtype)
-    if out is not main:
-        main.add_(out)
+        bf16 = w.dtype is torch.bfloat16
+        return torch.empty(w.shape, dtype=torch.bfloat16 if bf16 else torch.float32, device=w.device), not bf16
+    if main.dtype is torch.float32 and main.is_contiguous():
+        return main, _ADD
+    return torch.empty(w.shape, dtype=torch.float32, device=w.device), _FP32
+
+
+def _returned(w, out, mode):
+    """What autograd gets for ``w`` once ``_gradient_of``'s tensor is written."""
+    if mode == _ADD:
+        return None
+    main = None if mode == _BF16 else main_grad_of(w)
+    if main is None:
+        return out if out.dtype is w.dtype else out.to(w.dtype)
+    main.add_(out)
     return None
 
 
@@ -389,7 +391,7 @@ class _LinearFp8Block(torch.autograd.Function):
         _check_widths(T, K, N)
         with _on_device(x, w, bias):
             x2, w2 = _aligned(x2), _aligned(w)
-            if bias is not None:
+            if bias is not None and (bias.dtype is not torch.bfloat16 or not bias.is_contiguous()):
                 bias = bias.to(torch.bfloat16).contiguous()
             n_saved, n_tmp, _ = _linear_bytes(T, K, N, need)
             saved, tmp, at = _storage(n_saved, n_tmp, x.device)
@@ -404,14 +406,14 @@ class _LinearFp8Block(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        w = ctx.saved_tensors[0]
+        w, *kept = ctx.saved_tensors
         shape, x_dtype = ctx.x_like
         N, K = w.shape
         dy2 = _rows(dy, N)
         T, need = dy2.shape[0], ctx.need
         dx = dw = db = None
-        if len(ctx.saved_tensors) == 3:      # on the CPU
-            _, xv_t, wv = ctx.saved_tensors
+        if len(kept) == 2:      # on the CPU
+            xv_t, wv = kept
             dq, dq_t = _quantize_eager(dy2, False, False, True, True)
             if need & 1:
                 dx = (dq.dequantize() @ wv).view(shape).to(x_dtype)
@@ -420,24 +422,27 @@ class _LinearFp8Block(torch.autograd.Function):
             if need & 4:
                 db = dy2.float().sum(0).to(ctx.bias_dtype)
             return dx, dw, db
-        saved = ctx.saved_tensors[1]
+        saved, dev = kept[0], dy.device
         with _on_device(dy, w):
             dy2 = _aligned(dy2)
+            x_mode = x_dtype is torch.float32
             if need & 1:
-                dx = torch.empty(shape, dtype=torch.float32 if x_dtype == torch.float32 else torch.bfloat16,
-                                 device=dy.device)
-            g = _gradient_of(w) if need & 2 else (None, _BF16)
+                dx = torch.empty(shape, dtype=torch.float32 if x_mode else torch.bfloat16, device=dev)
+            g, g_mode = _gradient_of(w) if need & 2 else (None, _BF16)
+            b_mode = ctx.bias_dtype is not torch.bfloat16
             if need & 4:
-                db = torch.empty(N, dtype=torch.bfloat16 if ctx.bias_dtype == torch.bfloat16 else torch.float32,
-                                 device=dy.device)
-            x_mode = _FP32 if dx is not None and dx.dtype == torch.float32 else _BF16
-            tmp = _bytes(_linear_bytes(T, K, N, need)[2], dy.device)
+                db = torch.empty(N, dtype=torch.float32 if b_mode else torch.bfloat16, device=dev)
+            tmp = _bytes(_linear_bytes(T, K, N, need)[2], dev)
             _call("lb_linear_block_bwd", dy2.data_ptr(), dy2.stride(0), T, K, N, need, saved.data_ptr(), tmp.data_ptr(),
-                  nv.ptr(dx), x_mode, nv.ptr(g[0]), g[1], nv.ptr(db), 0 if db is None else _mode(db.dtype),
-                  _status_ptr(dy.device), nv.stream_ptr())
+                  nv.ptr(dx), x_mode, nv.ptr(g), g_mode, nv.ptr(db), b_mode, _status_ptr(dev), nv.stream_ptr())
             nv.count_launch(1 + bool(need & 1) + bool(need & 2) + bool(need & 4))
-            dw = _returned(w, g[0]) if need & 2 else None
-            return (None if dx is None else dx.to(x_dtype)), dw, (None if db is None else db.to(ctx.bias_dtype))
+            if need & 2:
+                dw = _returned(w, g, g_mode)
+            if need & 1 and dx.dtype is not x_dtype:
+                dx = dx.to(x_dtype)
+            if need & 4 and db.dtype is not ctx.bias_dtype:
+                db = db.to(ctx.bias_dtype)
+        return dx, dw, db
 
 
 def linear_fp8_block(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -472,7 +477,7 @@ def linear_fp8_block(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) ->
     _check_widths(T, K, N)
     with _on_device(x, w._data, bias):
         x2 = _aligned(x2)
-        if bias is not None:
+        if bias is not None and (bias.dtype is not torch.bfloat16 or not bias.is_contiguous()):
             bias = bias.to(torch.bfloat16).contiguous()
         y = torch.empty((T, N), dtype=act, device=x.device)
         n = _linear_kept_bytes(T, K, N)
@@ -555,15 +560,15 @@ class _GatedMlpFp8Block(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        w_gate, w_up, w_down = ctx.saved_tensors[:3]
+        w_gate, w_up, w_down, *kept = ctx.saved_tensors
         shape, x_dtype = ctx.x_like
         H, I = w_down.shape
         dy2 = _rows(dy, H)
         T, need = dy2.shape[0], ctx.need
         nx, ng, nu, nd = ctx.needs_input_grad[:4]
         dx = dg = du = dd = None
-        if len(ctx.saved_tensors) > 4:       # on the CPU
-            gu, h, xv_t, wv, dv = ctx.saved_tensors[3:]
+        if len(kept) > 1:       # on the CPU
+            gu, h, xv_t, wv, dv = kept
             dq, dq_t = _quantize_eager(dy2, False, False, True, True)
             dh = (dq.dequantize() @ dv).to(torch.bfloat16)
             d, d_t = _quantize_eager(_glu_grad_ref(gu[:, :I], gu[:, I:], dh, ctx.kind), False, False, True, True)
@@ -579,7 +584,7 @@ class _GatedMlpFp8Block(torch.autograd.Function):
                 h_t = _quantize_eager(h, False, False, False, True)[1].dequantize()
                 dd = (dq_t.dequantize() @ h_t.t()).to(w_down.dtype)
             return dx, dg, du, dd, None
-        saved = ctx.saved_tensors[3]
+        saved = kept[0]
         with _on_device(dy, w_down):
             dy2 = _aligned(dy2)
             dx = torch.empty(shape, dtype=torch.bfloat16, device=dy.device) if nx else None
@@ -592,9 +597,11 @@ class _GatedMlpFp8Block(torch.autograd.Function):
                   saved.data_ptr(), tmp.data_ptr(), nv.ptr(dx), *(nv.ptr(g[0]) for g in grads), ctypes.addressof(m),
                   _status_ptr(dy.device), nv.stream_ptr())
             nv.count_launch(2 + bool(need & 3) + nx + ng + nu + nd)
-            dg, du, dd = (_returned(w, g[0]) if n else None
+            dg, du, dd = (_returned(w, *g) if n else None
                           for w, n, g in zip((w_gate, w_up, w_down), (ng, nu, nd), grads))
-            return (None if dx is None else dx.to(x_dtype)), dg, du, dd, None
+            if nx and dx.dtype is not x_dtype:
+                dx = dx.to(x_dtype)
+        return dx, dg, du, dd, None
 
 
 def gated_mlp_fp8_block(x: torch.Tensor, w_gate, w_up, w_down, kind: str = "swiglu") -> torch.Tensor:
