@@ -4,6 +4,8 @@
 // In place of the per-tensor and per-row casts of fp8_cast.cu where the scales are those of blocks: a block
 // lies within a CTA's 128 x 128 tile, so the largest magnitude, the rounding and both layouts come from one
 // read, and there is no pass for the maxima.
+// Measured: 16384 x 4096 in both layouts 46 us (5.8 TB/s, 0.89 of copy bandwidth; with a scale and an unpacking for each
+// output, and every thread joining the warps' maxima, 62), the gated backward of 8192 x 4864 112 us (3.9 TB/s).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -354,6 +356,11 @@ __global__ void __launch_bounds__(512)
 // [T, 2 I], gate columns first) and of 128 tokens (`d_t` [2 I, T]), and h once more, in blocks of 128 tokens
 // (`h_t` [I, T]): the operands of the input gradient and of both weight gradients from one read. I is a
 // multiple of 128, so that no block holds columns of both. WANT: of the gradients' layouts; H: h.
+//
+// 11 bytes and 51 instructions a value: bound by those (54 % of the issue slots) and by the loads that two CTAs of an SM
+// leave uncovered. 16 warps of twice the values each (128 registers) took 128 us for the 112 of 8192 x 4864; a
+// persistent form that loads the next tile ahead spilled 700 bytes a thread and took 177; a prefetch of a later tile
+// into L2 109, with a quarter more read.
 constexpr int kGluSmem = sizeof(CastSmem<3>);
 template <int KIND, int WANT, int H>
 __global__ void __launch_bounds__(512, 2)

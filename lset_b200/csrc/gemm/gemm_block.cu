@@ -15,6 +15,11 @@
 // CAST: A is bf16 still, and warps 2-5 cast the blocks of its rows on their way into shared memory, each CTA those of
 // its own depth. For up to 32 rows, where a launch (3 us with its gap, and the host's 4) costs more than casting the
 // few rows in every CTA: 12 x 2560 x 4096 11.0 -> 8.1 us.
+//
+// Bound by launch, set-up and epilogue (3.6 us of an empty contraction in tiles of 16 rows, 8.2 in tiles of 128) and
+// then by the weights' way from memory: 12 x 19456 x 2560 in 12.4 us (4.0 TB/s), 12 x 2560 x 9728 in 10.1 split four
+// ways (19.4 whole). Sums go through shared memory so that a thread stores 16 bytes: as 2-byte stores from the
+// accumulator's lanes the epilogue of 128 rows took 7 us more.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -430,10 +435,6 @@ int launch_block(const CUtensorMap& tmP, const CUtensorMap& tmQ, const BlockArgs
                     stream, pdl_enabled(), splits, tmP, tmQ, g);
 }
 
-}  // namespace
-
-namespace {
-
 // What a launch takes apart from A.
 int block_args(BlockArgs& g, CUtensorMap* tmP, int tn, int splits, const BlockMat& B, void* C, int M, int N, int K,
                long long ldc, int out_fp32, int accumulate, const void* bias, int* status, long long* tiles) {
@@ -503,7 +504,7 @@ int block_gemm_cast(const BlockPlan& p, const void* x, long long ldx, const Bloc
                     : launch_block<32, 1>(tmP, tmP, g, tiles, p.splits, stream);
 }
 
-// Modelled time (us) of a product, fitted to 1300 runs of 100 sizes (rows 1 to 6144, columns 768 to 19456, depths 257
+// Modelled time (us) of a product, fitted to 887 runs of 116 sizes (rows 1 to 6144, columns 768 to 19456, depths 257
 // to 9728, every tile and split that fits, with what a launch costs in a CUDA graph): off by 17 % in the mean for the
 // one-CTA kernel, by 6 % for the pairs; the variant it chooses takes 1.5 % longer than the best in the mean and 19 % at
 // most. Measured at what the choice turns on: 128 x 2304 x 768 5.0 us in tiles of 16, 7.9 on pairs; 128 x 19456 x 2560

@@ -13,6 +13,12 @@
 //
 //   warp 0      TMA producer                  warps 2-9    epilogue
 //   warp 1      leader: MMA issuer            warps 10-13  scales
+//
+// Measured: 8192 x 4096 x 4096 95 us (2.88 PFLOP/s, the tensor pipe active in 78 % of the cycles), 20960 x 6144 x 4096
+// 355 us (2.97) when it runs by itself, 430 in a loop that the power limit slows. Bound by the tensor cores: a tile takes
+// 1.8 us and 2.4 us for each 1000 of depth (2.1 at their rate), the same with one scale a tensor, so what the scales
+// cost is not seen: 16384 x 4096 x 4096 205 us, 195 with a scale a tensor and two whole accumulators; 8192 x 8192 x 512,
+// which the epilogue bounds, 65 and 72.
 #include <cuda_bf16.h>
 
 #include "../common/pair.cuh"
@@ -212,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t scales = tmem_base + kScaleCols + 16 * slot;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
+            if (k >= 4 && st * BK + kScaleBlock >= g.K) break;   // no second block: nor is there a scale for it
             const uint32_t sf = uint32_t(2 * at + k / 4);
             umma2_block(d_tmem, umma_smem_desc(sa + (k / 4) * (BM * 128) + (k % 4) * 32, 16, 1024),
                         umma_smem_desc(sb + (k / 4) * (BNh * 128) + (k % 4) * 32, 16, 1024),

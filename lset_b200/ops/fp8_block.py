@@ -36,7 +36,8 @@ _MOST = 1 << 30      # rows and columns are counted in 32 bits
 class Fp8BlockTensor:
     """A matrix ``[rows, cols]`` in 8 bits: ``data`` ``[rows, ld]`` bytes (the first ``cols`` of a row are
     valid; ``ld`` a multiple of 16), ``scales`` ``[ceil(cols / 512), rows, 4]`` bytes: ``scales[b // 4, r,
-    b % 4]`` is the exponent, biased by 127, of the scale of columns ``128 b .. 128 b + 127`` of row ``r``.
+    b % 4]`` is the exponent (1 to 254, biased by 127) of the scale of columns ``128 b .. 128 b + 127`` of row ``r``;
+    bytes of blocks that a row does not have are not read.
 
     The two are checked here, once; a product takes them as they are.
     """
@@ -266,7 +267,8 @@ def matmul_fp8_block(a: Fp8BlockTensor, b: Fp8BlockTensor, *, out: Optional[torc
     """``C[M, N] = A · Bᵀ (+ bias)`` of block-scaled ``a [M, K]`` and ``b [N, K]``, in bf16 or fp32.
 
     ``out`` may be given (rows of unit inner stride); ``accumulate`` adds into it (fp32, no bias). Sums are
-    fp32 and their order depends on the sizes alone. e4m3 and e5m2 operands may be mixed.
+    fp32, in an order that the sizes and whether ``out``'s rows start at multiples of 16 bytes decide, and nothing
+    else. e4m3 and e5m2 operands may be mixed.
     """
     M, N, K = a.rows, b.rows, a.cols
     if b.cols != K:

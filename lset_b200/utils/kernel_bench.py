@@ -4,6 +4,7 @@ captures under ``profiles/`` are taken from).
     python -m lset_b200.utils.kernel_bench gemm  --m 23040 --n 4096 --k 1024 [--form fprop|dgrad|wgrad]
                                                  [--ref torch]   (torch.matmul / cuBLAS alongside)
     python -m lset_b200.utils.kernel_bench fp8   --m 23040 --n 4096 --k 1024 [--what gemm|cast|linear]
+                                                 [--block]   (a scale for each block of 128)
     python -m lset_b200.utils.kernel_bench attn  --seqs 64 --len 320 --hq 16 --hk 8 --hd 128 [--bwd]
                                                  [--ref flash]   (flash_attn_varlen_func alongside)
     python -m lset_b200.utils.kernel_bench norm  --rows 23040 --h 1024 [--bwd]
@@ -91,6 +92,8 @@ def bench_fp8(a):
 
     M, N, K = a.m, a.n, a.k
     x, w = _r(M, K), _r(N, K)
+    if a.block:
+        return _bench_fp8_block(a, x, w)
     mode = f8.PER_ROW if a.rowwise else f8.PER_TENSOR
     xq, _ = f8.quantize_fp8(x, mode)
     wq, _ = f8.quantize_fp8(w, mode)
@@ -110,6 +113,29 @@ def bench_fp8(a):
     ms_bf16 = _time(lambda: matmul_abt(x, w), a.iters)
     return dict(kernel=f"fp8_{a.what}", rowwise=bool(a.rowwise), M=M, N=N, K=K, ms=ms,
                 bf16_gemm_ms=ms_bf16, **roofline(ms, flops, byt))
+
+
+def _bench_fp8_block(a, x, w):
+    """The same with a scale for each block of 128 (``linear``: the layer on a kept weight)."""
+    import torch
+
+    from ..ops import fp8_block as fb
+    from ..ops.gemm import matmul_abt
+
+    M, N, K = a.m, a.n, a.k
+    (xq, _), (wq, _) = fb.quantize_fp8_block(x), fb.quantize_fp8_block(w, tile=True)
+    flops, byt = 2.0 * M * N * K, 1.0 * (M * K + N * K) + 2.0 * M * N
+    if a.what == "gemm":
+        fn = lambda: fb.matmul_fp8_block(xq, wq)  # noqa: E731
+    elif a.what == "cast":
+        fn = lambda: fb.quantize_fp8_block(x, want_t=True)  # noqa: E731
+        flops, byt = 0.0, 4.0 * M * K
+    else:
+        fn = lambda: fb.linear_fp8_block(x, wq)  # noqa: E731
+        byt += 1.0 * M * K
+    with torch.no_grad():
+        ms, ms_bf16 = _time(fn, a.iters), _time(lambda: matmul_abt(x, w), a.iters)
+    return dict(kernel=f"fp8_block_{a.what}", M=M, N=N, K=K, ms=ms, bf16_gemm_ms=ms_bf16, **roofline(ms, flops, byt))
 
 
 def bench_attn(a):
@@ -299,7 +325,7 @@ def main(argv=None):
     f = sub.add_parser("fp8")
     f.add_argument("--m", type=int, default=23040); f.add_argument("--n", type=int, default=4096)
     f.add_argument("--k", type=int, default=1024); f.add_argument("--what", default="gemm")
-    f.add_argument("--rowwise", action="store_true")
+    f.add_argument("--rowwise", action="store_true"); f.add_argument("--block", action="store_true")
     t = sub.add_parser("attn")
     t.add_argument("--seqs", type=int, default=64); t.add_argument("--len", type=int, default=320)
     t.add_argument("--hq", type=int, default=16); t.add_argument("--hk", type=int, default=8)

@@ -123,6 +123,19 @@ def test_parts_of_a_cast_matrix():
         _check_product(fb.matmul_fp8_block(a, part), a, part)
 
 
+@pytest.mark.parametrize("M,N,K", [(5, 136, 272), (300, 264, 640), (1500, 2056, 640), (2000, 2304, 16)])
+def test_bytes_of_blocks_that_are_not_there_are_not_read(M, N, K):
+    a, _ = fb.quantize_fp8_block(_rand(M, K))
+    b, _ = fb.quantize_fp8_block(_rand(N, K, seed=1), tile=True)
+    want = fb.matmul_fp8_block(a, b)
+    for q in (a, b):
+        words = q.scales.transpose(0, 1).reshape(q.rows, -1).clone()
+        words[:, (K + 127) // 128:] = 255          # not a number
+        q.scales.copy_(words.view(q.rows, -1, 4).transpose(0, 1))
+        q.data[:, K:] = 0x7F
+    assert torch.equal(fb.matmul_fp8_block(a, b), want)
+
+
 def test_values_that_are_not_finite_stay_in_their_rows():
     x = _rand(6, 384)
     x[2, 130], x[4, 0] = float("nan"), float("inf")
