@@ -42,10 +42,9 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = 32 * (2 + kEpiWarps + 4);
 constexpr int EPI_WORDS = 32 * 33;
 constexpr int kBarBytes = 512;
-constexpr int kTops = 32 * 80;               // GLU: where a warp's largest magnitudes lie, behind its 32 staged rows
 constexpr int SMEM_BYTES = kStages * STAGE_BYTES + 1024 + kBarBytes + kEpiWarps * EPI_WORDS * 4;
 constexpr int kAcc1 = 224, kScaleCols = 480, kSlots = 2;
-static_assert(SMEM_BYTES <= 232448 && kTops + 2 * 32 * 4 <= EPI_WORDS * 4, "");
+static_assert(SMEM_BYTES <= 232448, "");
 
 struct Block2Args {
   int M, N, K;
@@ -53,6 +52,7 @@ struct Block2Args {
   long long rows_sa, rows_sb;
   void* C;                                   // GLU: gate products (null: not wanted)
   long long ldc;
+  int wide, wide_h;                          // rows of C (GLU: of both products), of h start at multiples of 32 bytes
   int accumulate;                            // fp32 only: C += result
   const __nv_bfloat16* bias;
   int a_e5m2, b_e5m2;
@@ -79,6 +79,27 @@ __device__ __forceinline__ void umma2_block(uint32_t tmem_d, uint64_t adesc, uin
       :
       : "r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(tmem_sa), "r"(tmem_sb), "r"(accumulate)
       : "memory");
+}
+
+// 32 bytes, a whole sector, from one lane.
+__device__ __forceinline__ void st32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+// A lane's WORDS words of a row, the first `bytes` of them (a multiple of 16); wide: at a multiple of 32.
+template <int WORDS>
+__device__ __forceinline__ void store_words(void* dst, const uint32_t (&w)[WORDS], int bytes, bool wide) {
+  uint8_t* p = static_cast<uint8_t*>(dst);
+  if (wide && bytes >= 4 * WORDS) {
+#pragma unroll
+    for (int j = 0; j < WORDS / 8; ++j) st32(p + 32 * j, w + 8 * j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < WORDS / 4; ++j)
+      if (16 * j < bytes)
+        *reinterpret_cast<uint4*>(p + 16 * j) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+  }
 }
 
 template <typename OutT, int GLU>
@@ -319,7 +340,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       if constexpr (GLU) {
         uint32_t h[2][16];
         uint32_t top = 0u;
-        const int rr = lane >> 2, cc = lane & 3;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int c = 2 * half + ((i + rot) & 1);
@@ -350,27 +370,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
 #pragma unroll
           for (int j = 0; j < 16; ++j) top = __vmaxu2(top, h[i][j] & 0x7fff7fffu);
-          if (g.C != nullptr) {
-#pragma unroll
-            for (int o = 0; o < 2; ++o) {
-              OutT* dst = reinterpret_cast<OutT*>(o == 0 ? g.C : g.up_out);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                *reinterpret_cast<uint4*>(sblk + lane * 80 + 16 * j) =
-                    make_uint4(w[o][4 * j], w[o][4 * j + 1], w[o][4 * j + 2], w[o][4 * j + 3]);
-              __syncwarp();
-              const int f0 = n0 + c * 32 + cc * 8;
-              if (f0 < g.N) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const int lr = k * 8 + rr, grow = m0 + q * 32 + lr;
-                  if (grow < g.M)
-                    *reinterpret_cast<uint4*>(dst + grow * g.ldc + f0) =
-                        *reinterpret_cast<const uint4*>(sblk + lr * 80 + cc * 16);
-                }
-              }
-              __syncwarp();
-            }
+          if (g.C != nullptr && row < g.M) {
+            const long long at = row * g.ldc + n0 + c * 32;
+            store_words(reinterpret_cast<OutT*>(g.C) + at, w[0], 64, g.wide);
+            store_words(reinterpret_cast<OutT*>(g.up_out) + at, w[1], 64, g.wide);
           }
         }
         tc_fence_before();
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) mbar_arrive_remote(acc ? tempty1 : tempty0);
         // a block of a row is this tile's 128 features: the largest magnitude of both halves
         top = max(top & 0xffffu, top >> 16);
-        uint32_t* tops = reinterpret_cast<uint32_t*>(sblk + kTops) + acc * 32 + lane;   // two tiles in turn
+        uint32_t* tops = reinterpret_cast<uint32_t*>(sblk) + acc * 32 + lane;   // two tiles in turn
         *tops = top;
         asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
         top = max(top, tops[half ? -4 * EPI_WORDS : 4 * EPI_WORDS]);   // the warp with the other half of the rows
@@ -393,9 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float2 a = unpack_bf16x2(h[i][2 * j]), b = unpack_bf16x2(h[i][2 * j + 1]);
               o[j] = cast4<0>(a.x * s, a.y * s, b.x * s, b.y * s);
             }
-            uint4* dst = reinterpret_cast<uint4*>(g.h + row * g.ldh + f0);
-            dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-            dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+            store_words(g.h + row * g.ldh + f0, o, 32, g.wide_h);
           }
           if (half == 0) {
             const int kb = n0 / kScaleBlock;
@@ -426,25 +427,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               r[j] = __float_as_uint(__uint_as_float(r[j]) + __shfl_sync(0xffffffffu, b, j));
           }
           if constexpr (sizeof(OutT) == 2) {
+            uint32_t w[16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<uint4*>(sblk + lane * 80 + 16 * j) = make_uint4(
-                  pack_bf16x2(__uint_as_float(r[8 * j]), __uint_as_float(r[8 * j + 1])),
-                  pack_bf16x2(__uint_as_float(r[8 * j + 2]), __uint_as_float(r[8 * j + 3])),
-                  pack_bf16x2(__uint_as_float(r[8 * j + 4]), __uint_as_float(r[8 * j + 5])),
-                  pack_bf16x2(__uint_as_float(r[8 * j + 6]), __uint_as_float(r[8 * j + 7])));
-            __syncwarp();
-            const int rr = lane >> 2, cc = lane & 3;
-            if (col0 + cc * 8 < g.N) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const int lr = k * 8 + rr, grow = m0 + q * 32 + lr;
-                if (grow < g.M)
-                  *reinterpret_cast<uint4*>(Cout + grow * g.ldc + col0 + cc * 8) =
-                      *reinterpret_cast<const uint4*>(sblk + lr * 80 + cc * 16);
-              }
-            }
-            __syncwarp();
+            for (int j = 0; j < 16; ++j)
+              w[j] = pack_bf16x2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1]));
+            if (row < g.M) store_words(Cout + row * g.ldc + col0, w, 2 * (g.N - col0), g.wide);
+          } else if (!g.accumulate) {
+            if (row < g.M) store_words(Cout + row * g.ldc + col0, r, 4 * (g.N - col0), g.wide);
           } else {
             float* st = reinterpret_cast<float*>(sblk);
 #pragma unroll
@@ -455,14 +444,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int k = 0; k < 8; ++k) {
                 const int lr = k * 4 + rr, grow = m0 + q * 32 + lr;
-                if (grow < g.M) {
-                  const float* sp = st + lr * 33 + cc;
-                  float* dst = reinterpret_cast<float*>(Cout) + grow * g.ldc + col0 + cc;
-                  if (g.accumulate)   // one tile adds to an element: the order of tiles does not matter
-                    red_add4(dst, sp[0], sp[1], sp[2], sp[3]);
-                  else
-                    *reinterpret_cast<float4*>(dst) = make_float4(sp[0], sp[1], sp[2], sp[3]);
-                }
+                const float* sp = st + lr * 33 + cc;
+                if (grow < g.M)   // one tile adds to an element: the order of tiles does not matter
+                  red_add4(reinterpret_cast<float*>(Cout) + grow * g.ldc + col0 + cc, sp[0], sp[1], sp[2], sp[3]);
               }
             }
             __syncwarp();
@@ -562,6 +546,7 @@ int block_gemm_2cta(int splits, long long split_stride, const BlockMat& A, const
   g.rows_sb = B.rows_s;
   g.C = C;
   g.ldc = ldc;
+  g.wide = !(reinterpret_cast<uintptr_t>(C) & 31) && !(ldc & (out_fp32 ? 7 : 15));
   g.accumulate = accumulate;
   g.bias = static_cast<const __nv_bfloat16*>(bias);
   g.a_e5m2 = A.e5m2 ? 1 : 0;
@@ -569,6 +554,7 @@ int block_gemm_2cta(int splits, long long split_stride, const BlockMat& A, const
   g.splits = splits;
   g.stages_per_split = stages_of_split(K, splits);
   g.split_stride = splits > 1 ? split_stride : 0;
+  if (g.split_stride & 7) g.wide = 0;
   g.band = band_of(tiles_n, 1LL * N * K);
   g.status = status;
   const long long total = 1LL * tiles_m * tiles_n * splits;
@@ -602,6 +588,8 @@ int block_gemm_glu(int kind, const BlockMat& A, const BlockMat& Wg, const BlockM
   g.C = gate;
   g.up_out = up;
   g.ldc = ld_gu;
+  g.wide = !(reinterpret_cast<uintptr_t>(gate) & 31) && !(reinterpret_cast<uintptr_t>(up) & 31) && !(ld_gu & 15);
+  g.wide_h = !(reinterpret_cast<uintptr_t>(h.data) & 31) && !(h.ld & 31);
   g.a_e5m2 = A.e5m2 ? 1 : 0;
   g.b_e5m2 = Wg.e5m2 ? 1 : 0;
   g.splits = 1;
