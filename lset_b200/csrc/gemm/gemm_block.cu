@@ -526,8 +526,10 @@ static float cost_1cta(int M, int N, int K, int tn, int splits) {
 static float cost_2cta(int M, int N, int K, int splits) {
   constexpr float pairs = 74.f;
   const float tiles = 1.f * ((M + 255) / 256) * ((N + 255) / 256) * splits;
-  const float each = 1e-3f * K / splits;
-  return 4.85f + ceilf(tiles / pairs) * (1.83f + 2.4f * each) +
+  const float each = 1e-3f * K / splits, full = floorf(tiles / pairs), rest = tiles - full * pairs;
+  // (a last wave of few tiles runs in halves)
+  const float waves = full + (rest == 0.f ? 0.f : (splits == 1 && 2.f * rest <= pairs ? 0.55f : 1.f));
+  return 4.85f + waves * (1.83f + 2.4f * each) +
          (splits > 1 ? 3.35f + 0.6e-6f * splits * M * float(N) : 0.f);
 }
 

@@ -59,6 +59,7 @@ struct Block2Args {
   int splits, stages_per_split;
   long long split_stride;                    // elements between the outputs of two splits
   int band;                                  // rows of tiles in a band; 0: row by row
+  int whole, items;                          // work items: `whole` tiles, then halves of 128 columns
   void* up_out;                              // GLU: up products, and act(gate) * up cast in blocks of a row
   uint8_t* h;
   long long ldh;
@@ -158,10 +159,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr int kTileN = GLU ? BNh : BNp;   // output columns (features) of a tile
   const int tiles_m = (g.M + 2 * BM - 1) / (2 * BM), tiles_n = (g.N + kTileN - 1) / kTileN;
   const int stages_total = (g.K + BK - 1) / BK;
-  const int total = tiles_m * tiles_n * g.splits;
+  const int total = g.items;
   const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   // Tiles row by row or in bands (band_of in gemm_2cta.cu says why). m0: first row of this CTA's half.
-  auto decode = [&](int tile, int& split, int& m0, int& n0, int& st0, int& st1) {
+  // narrow: an item of 128 columns, half a tile.
+  bool narrow = false;
+  auto decode = [&](int item, int& split, int& m0, int& n0, int& st0, int& st1) {
+    narrow = !GLU && item >= g.whole;
+    const int tile = narrow ? g.whole + (item - g.whole) / 2 : item;
     split = tile / (tiles_m * tiles_n);
     const int mn = tile - split * (tiles_m * tiles_n);
     int mt = mn / tiles_n, nt = mn - mt * tiles_n;
@@ -172,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mt = first + at - nt * rows;
     }
     m0 = mt * (2 * BM) + int(rank) * BM;
-    n0 = nt * kTileN;
+    n0 = nt * kTileN + (narrow ? ((item - g.whole) & 1) * BNh : 0);
     st0 = split * g.stages_per_split;
     st1 = min(st0 + g.stages_per_split, stages_total);
   };
@@ -186,22 +191,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int tile = pair; tile < total && ok; tile += npairs) {
         decode(tile, split, m0, n0, st0, st1);
-        const int nb = GLU ? n0 : n0 + int(rank) * BNh;
-        const CUtensorMap* tb = GLU && !leader ? &tmB2 : &tmB;
+        // (GLU: tmB2 is the up weight; else B in boxes of 64 rows, for narrow items)
+        const int rows = narrow ? BNh / 2 : BNh;
+        const int nb = GLU ? n0 : n0 + int(rank) * rows;
+        const CUtensorMap* tb = (GLU ? !leader : narrow) ? &tmB2 : &tmB;
         for (int st = st0; st < st1; ++st) {
           if (!mbar_wait(&empty[stage], phase ^ 1u)) {
             report_status(g.status, kStatusTimeoutProducer);
             ok = false;
             break;
           }
-          if (leader) mbar_expect_tx(&full[stage], 2 * STAGE_BYTES);
+          if (leader) mbar_expect_tx(&full[stage], 2 * (A_BYTES + rows * BK));
           uint8_t* sa = smem + stage * STAGE_BYTES;
           uint8_t* sb = sa + A_BYTES;
           const uint32_t bar = map_to_cta(&full[stage], 0);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             tma_load_2d_pair(sa + h * (BM * 128), &tmA, bar, st * BK + 128 * h, m0);
-            tma_load_2d_pair(sb + h * (BNh * 128), tb, bar, st * BK + 128 * h, nb);
+            tma_load_2d_pair(sb + h * (rows * 128), tb, bar, st * BK + 128 * h, nb);
           }
           if (++stage == kStages) {
             stage = 0;
@@ -214,7 +221,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 1) {
     if (leader && elect_one()) {
       // ---------------------------------------------------------------- MMA issuer (leader)
-      const uint32_t idesc0 = umma_idesc_block(2 * BM, BNp, g.a_e5m2, g.b_e5m2, 0);
       int stage = 0, group = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -227,6 +233,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (acc ? kAcc1 : 0);
+        const uint32_t idesc0 = umma_idesc_block(2 * BM, narrow ? BNh : BNp, g.a_e5m2, g.b_e5m2, 0);
+        const uint32_t b_half = narrow ? BNh / 2 * 128 : BNh * 128;   // bytes of 128 of depth
         for (int st = st0; st < st1; ++st) {
           const int at = (st - st0) % kGroup, slot = group % kSlots;
           if ((at == 0 && !mbar_wait(&sfull[slot], (group / kSlots) & 1)) || !mbar_wait(&full[stage], phase)) {
@@ -242,7 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (k >= 4 && st * BK + kScaleBlock >= g.K) break;   // no second block: nor is there a scale for it
             const uint32_t sf = uint32_t(2 * at + k / 4);
             umma2_block(d_tmem, umma_smem_desc(sa + (k / 4) * (BM * 128) + (k % 4) * 32, 16, 1024),
-                        umma_smem_desc(sb + (k / 4) * (BNh * 128) + (k % 4) * 32, 16, 1024),
+                        umma_smem_desc(sb + (k / 4) * b_half + (k % 4) * 32, 16, 1024),
                         idesc0 | (sf << 4) | (sf << 29), scales, scales + 4, st > st0 || k > 0);
           }
           umma2_commit_both(&empty[stage], 1u);
@@ -408,9 +416,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       } else {
         OutT* Cout = reinterpret_cast<OutT*>(g.C) + split * g.split_stride;
+        const int chunks = narrow ? 2 : 4;   // of 32 columns, a half of the warps
 #pragma unroll 1
-        for (int i = 0; i < 4; ++i) {
-          const int c = 4 * half + ((i + rot) & 3);
+        for (int i = 0; i < chunks; ++i) {
+          const int c = chunks * half + ((i + rot) & (chunks - 1));
           uint32_t r[32];
           tmem_ld_32x32b_x32(src0 + c * 32, r);
           tmem_ld_wait();
@@ -472,7 +481,7 @@ constexpr int kMaxDevices = 64;
 int g_pairs[kMaxDevices];   // CTA pairs resident at once; 0: not asked yet
 
 template <typename OutT, int GLU>
-int launch_2cta(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2, const Block2Args& g,
+int launch_2cta(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2, Block2Args& g,
                 long long total, cudaStream_t stream) {
   auto kern = gemm_block_2cta_kernel<OutT, GLU>;
   static bool configured[kMaxDevices] = {};
@@ -503,7 +512,16 @@ int launch_2cta(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMa
     }
     g_pairs[dev] = n;
   }
-  const int pairs = int(total < g_pairs[dev] ? total : g_pairs[dev]);
+  // The tiles of the last wave in halves, where those still fit in one. (No sum changes with it.) Measured with whole
+  // tiles / halves: 6144 x 2560 x 8191 (240 tiles on 74 pairs) 123 / 99 us by itself; a training step of the linear layer
+  // 8191 x 2560 -> 6144, at the power limit, 419 / 405; of 16384 x 4096 -> 4096 837 / 844, of 16384 x 2560 x 9728 the same.
+  const int rest = int(total % g_pairs[dev]);
+  g.whole = g.items = int(total);
+  if (!GLU && g.splits == 1 && rest > 0 && 2 * rest <= g_pairs[dev]) {
+    g.whole = int(total) - rest;
+    g.items = g.whole + 2 * rest;
+  }
+  const int pairs = g.items < g_pairs[dev] ? g.items : g_pairs[dev];
   return launch_pdl(kern, dim3(2 * pairs), dim3(kThreads), SMEM_BYTES, stream, pdl_enabled(), 2, tmA, tmB, tmB2, g);
 }
 
@@ -530,10 +548,12 @@ int block_gemm_2cta(int splits, long long split_stride, const BlockMat& A, const
   if ((N & 7) || (ldc & 7) || (reinterpret_cast<uintptr_t>(C) & 15)) return -5;
   if (splits > 1 && (!out_fp32 || accumulate || bias != nullptr)) return -5;
   if (splits < 1 || !block_2cta_splits_ok(K, splits)) return -5;
-  CUtensorMap tmA, tmB;
+  CUtensorMap tmA, tmB, tmBh;
   int rc = make_tmap_2d(&tmA, A.data, 1, (uint64_t)K, (uint64_t)M, (uint64_t)A.ld, 128, BM, true);
   if (rc) return rc;
   rc = make_tmap_2d(&tmB, B.data, 1, (uint64_t)K, (uint64_t)N, (uint64_t)B.ld, 128, BNh, true);
+  if (rc) return rc;
+  rc = make_tmap_2d(&tmBh, B.data, 1, (uint64_t)K, (uint64_t)N, (uint64_t)B.ld, 128, BNh / 2, true);
   if (rc) return rc;
   const int tiles_m = (M + 2 * BM - 1) / (2 * BM), tiles_n = (N + BNp - 1) / BNp;
   Block2Args g{};
@@ -559,8 +579,8 @@ int block_gemm_2cta(int splits, long long split_stride, const BlockMat& A, const
   g.status = status;
   const long long total = 1LL * tiles_m * tiles_n * splits;
   if (total > 0x7fff0000LL) return -3;   // (tiles are counted in steps of the grid)
-  return out_fp32 ? launch_2cta<float, 0>(tmA, tmB, tmB, g, total, stream)
-                  : launch_2cta<__nv_bfloat16, 0>(tmA, tmB, tmB, g, total, stream);
+  return out_fp32 ? launch_2cta<float, 0>(tmA, tmB, tmBh, g, total, stream)
+                  : launch_2cta<__nv_bfloat16, 0>(tmA, tmB, tmBh, g, total, stream);
 }
 
 // gate and up weights [I, K], I a multiple of 128, with a common row stride and scale words of common groups. Both

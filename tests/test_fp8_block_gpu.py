@@ -70,7 +70,9 @@ SHAPES = [(1, 128, 128), (1, 8, 16), (5, 264, 272), (16, 128, 1024), (17, 136, 5
           (12, 4096, 2560), (1000, 1032, 1040),
           # tiles of CTA pairs: one stage, whole and ragged ones, more tiles than pairs, bands of them
           (1030, 2304, 16), (1500, 2056, 256), (2000, 2304, 640), (2561, 1288, 1040), (4097, 4360, 2576),
-          (1100, 16392, 2064)]
+          (1100, 16392, 2064),
+          # last waves in half tiles: of one wave, behind whole ones, with halves that lie outside the matrix
+          (4000, 264, 2048), (2300, 1024, 1040), (5000, 4096, 272), (9000, 2056, 640)]
 
 
 @pytest.mark.parametrize("M,N,K", SHAPES)
