@@ -14,11 +14,10 @@
 //   warp 0      TMA producer                  warps 2-9    epilogue
 //   warp 1      leader: MMA issuer            warps 10-13  scales
 //
-// Measured: 8192 x 4096 x 4096 95 us (2.88 PFLOP/s, the tensor pipe active in 78 % of the cycles), 20960 x 6144 x 4096
-// 355 us (2.97) when it runs by itself, 430 in a loop that the power limit slows. Bound by the tensor cores: a tile takes
-// 1.8 us and 2.4 us for each 1000 of depth (2.1 at their rate), the same with one scale a tensor, so what the scales
-// cost is not seen: 16384 x 4096 x 4096 205 us, 195 with a scale a tensor and two whole accumulators; 8192 x 8192 x 512,
-// which the epilogue bounds, 65 and 72.
+// Measured by itself, L2 flushed: 8192 x 4096 x 4096 92 us (2.98 PFLOP/s, the tensor pipe active in 81 % of the cycles),
+// 20960 x 6144 x 4096 334 us (3.16; 360 inside the layer), 16384 x 4096 x 4096 168 (3.27). Bound by the tensor cores where
+// the contraction is deep, and by the power limit over seconds; by the epilogue where it is short (8192 x 8192 x 512 45 us).
+// Rows stored from registers, for staging them in shared memory: 95.6 -> 92.9 us under the profiler at the first size.
 #include <cuda_bf16.h>
 
 #include "../common/pair.cuh"
@@ -512,9 +511,9 @@ int launch_2cta(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMa
     }
     g_pairs[dev] = n;
   }
-  // The tiles of the last wave in halves, where those still fit in one. (No sum changes with it.) Measured with whole
-  // tiles / halves: 6144 x 2560 x 8191 (240 tiles on 74 pairs) 123 / 99 us by itself; a training step of the linear layer
-  // 8191 x 2560 -> 6144, at the power limit, 419 / 405; of 16384 x 4096 -> 4096 837 / 844, of 16384 x 2560 x 9728 the same.
+  // The tiles of the last wave in halves, where those still fit in one. (No sum changes with it.) Measured in turn with
+  // whole tiles / halves, at the power limit: a training step of the linear layer 8191 x 2560 -> 6144 (its weight gradient
+  // has 240 tiles on 74 pairs) 403 / 394 us, of 16384 x 4096 -> 4096 788 / 788.
   const int rest = int(total % g_pairs[dev]);
   g.whole = g.items = int(total);
   if (!GLU && g.splits == 1 && rest > 0 && 2 * rest <= g_pairs[dev]) {
