@@ -61,16 +61,18 @@ struct Call {
     first = false;
   }
   void product(const BlockMat& a, const BlockMat& b, const Out& out, int M, int N, int K, long long ldc,
-               const void* bias = nullptr) {
+               const void* bias = nullptr, int deepest = 0) {
     run([&] {
-      const BlockPlan p = block_plan(M, N, K, aligned16(out.p) && !(N & 7) && !(ldc & 7));
+      const BlockPlan p = block_plan(M, N, K, aligned16(out.p) && !(N & 7) && !(ldc & 7), deepest);
       return block_gemm(p, a, b, out.p, M, N, K, ldc, out.mode > 0, out.mode == 2, bias, ws, status, stream);
     });
   }
 };
 
 // Storage of a product whatever the alignment of its output.
-size_t product_bytes(int M, int N, int K) { return block_plan_bytes(block_plan(M, N, K, !(N & 7)), M, N); }
+size_t product_bytes(int M, int N, int K, int deepest = 0) {
+  return block_plan_bytes(block_plan(M, N, K, !(N & 7), deepest), M, N);
+}
 size_t max2(size_t a, size_t b) { return a > b ? a : b; }
 
 struct LinearStorage {
@@ -119,7 +121,7 @@ MlpStorage mlp_storage(int T, int H, int I, int need, void* saved, void* tmp) {
   s.w = fwd.mat(2LL * I, H);
   s.wd = fwd.mat(H, I);
   s.h = fwd.mat(T, I);
-  s.ws_fwd = fwd.take(max2(product_bytes(T, 2 * I, H), product_bytes(T, H, I)));
+  s.ws_fwd = fwd.take(max2(product_bytes(T, 2 * I, H, kDeepestSum), product_bytes(T, H, I)));
   if (need_x || need_gu) {
     s.dy = bwd.mat(T, H);
     s.dh = static_cast<__nv_bfloat16*>(bwd.take(size_t(T) * I * 2));
@@ -129,7 +131,7 @@ MlpStorage mlp_storage(int T, int H, int I, int need, void* saved, void* tmp) {
   if (need_gu) s.d_t = bwd.mat(2LL * I, T);
   if (need_d) s.h_t = bwd.mat(I, T);
   size_t ws = 0;
-  if (need_x || need_gu) ws = max2(ws, product_bytes(T, I, H));
+  if (need_x || need_gu) ws = max2(ws, product_bytes(T, I, H, kDeepestSum));
   if (need_x) ws = max2(ws, product_bytes(T, H, 2 * I));
   if (need_gu) ws = max2(ws, max2(product_bytes(2 * I, H, T), product_bytes(I, H, T)));
   if (need_d) ws = max2(ws, product_bytes(H, I, T));
@@ -141,17 +143,19 @@ MlpStorage mlp_storage(int T, int H, int I, int need, void* saved, void* tmp) {
 }
 
 // y = (act(x Wgᵀ) * (x Wuᵀ)) Wdᵀ from cast operands. The two products stay in s.gu for the backward, are dropped, or
-// are there already.
+// are there already. What the backward reads is summed in parts (kDeepestSum); an encoder's gate and up products
+// go through h into one row of y alone, where a step of one value is lost among those of the row's others.
 enum GateUp { kKeepProducts, kDropProducts, kHaveProducts };
 void mlp_products(Call& c, int kind, const MlpStorage& s, int T, int H, int I, GateUp gu, void* y) {
   const bool keep = gu == kKeepProducts;
-  if (gu != kHaveProducts && block_glu_fused(T, I, H)) {
+  const int deepest = keep ? kDeepestSum : 0;
+  if (gu != kHaveProducts && block_glu_fused(T, I, H, deepest)) {
     c.run([&] {
-      return block_gemm_glu(kind, s.x, s.w, rows_of(s.w, I), T, I, H, keep ? s.gu : nullptr,
+      return block_gemm_glu(kind, deepest, s.x, s.w, rows_of(s.w, I), T, I, H, keep ? s.gu : nullptr,
                             keep ? s.gu + I : nullptr, 2LL * I, s.h, c.status, c.stream);
     });
   } else {
-    if (gu != kHaveProducts) c.product(s.x, s.w, Out{s.gu, 0}, T, 2 * I, H, 2LL * I);
+    if (gu != kHaveProducts) c.product(s.x, s.w, Out{s.gu, 0}, T, 2 * I, H, 2LL * I, nullptr, deepest);
     c.run([&] { return block_glu_fwd(kind, s.gu, s.gu + I, 2LL * I, T, I, s.h, c.stream); });
   }
   c.product(s.h, s.wd, Out{y, 0}, T, H, I, H);
@@ -265,14 +269,14 @@ extern "C" int lb_mlp_block_fwd(int kind, const void* x, long long ldx, const vo
 namespace {
 // Whether the gate and up product casts x itself.
 bool mlp_casts_itself(int T, int H, int I, const BlockPlan& p) {
-  return !block_glu_fused(T, I, H) && block_casts_itself(p, T, H);
+  return !block_glu_fused(T, I, H, 0) && block_casts_itself(p, T, H);
 }
 MlpStorage mlp_kept_storage(int T, int H, int I, bool cast_x, void* tmp) {
   MlpStorage s{};
   Arena a(tmp);
   if (!cast_x) s.x = a.mat(T, H);
   s.h = a.mat(T, I);
-  if (!block_glu_fused(T, I, H)) s.gu = static_cast<__nv_bfloat16*>(a.take(size_t(T) * 2 * I * 2));
+  if (!block_glu_fused(T, I, H, 0)) s.gu = static_cast<__nv_bfloat16*>(a.take(size_t(T) * 2 * I * 2));
   s.ws_fwd = a.take(max2(product_bytes(T, 2 * I, H), product_bytes(T, H, I)));
   s.fwd = a.at;
   return s;
@@ -311,7 +315,7 @@ extern "C" int lb_mlp_block_bwd(int kind, const void* dy, long long lddy, int T,
   Call c{status, reinterpret_cast<cudaStream_t>(stream_), s.ws_bwd};
   c.run([&] { return block_cast(dy, T, H, lddy, 0, 0, s.dy, s.dy_t, 0, nullptr, c.stream); });
   const bool inner = need & 3;
-  if (inner) c.product(s.dy, s.wd_t, Out{s.dh, 0}, T, I, H, I);
+  if (inner) c.product(s.dy, s.wd_t, Out{s.dh, 0}, T, I, H, I, nullptr, kDeepestSum);
   c.run([&] {
     // (for h alone the gradient is not used; anything of its size will do)
     return block_glu_bwd(kind, inner ? s.dh : s.gu, inner ? I : 2LL * I, s.gu, s.gu + I, 2LL * I, T, I, s.d, s.d_t,

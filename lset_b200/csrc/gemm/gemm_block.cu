@@ -523,41 +523,44 @@ static float cost_1cta(int M, int N, int K, int tn, int splits) {
 }
 // (The plan depends on the sizes alone, not on the device's count of pairs: storage is sized by it, and it fixes the
 // order of sums.)
-static float cost_2cta(int M, int N, int K, int splits) {
+static float cost_2cta(int M, int N, int K, int splits, int deepest) {
   constexpr float pairs = 74.f;
   const float tiles = 1.f * ((M + 255) / 256) * ((N + 255) / 256) * splits;
   const float each = 1e-3f * K / splits, full = floorf(tiles / pairs), rest = tiles - full * pairs;
   // (a last wave of few tiles runs in halves)
   const float waves = full + (rest == 0.f ? 0.f : (splits == 1 && 2.f * rest <= pairs ? 0.55f : 1.f));
-  return 4.85f + waves * (1.83f + 2.4f * each) +
+  // (the issuer waits for the end of a sum and the first of its columns before it starts the next: 0.6 to 0.8 us)
+  const float joins = 0.6f * (block_2cta_sums(K, deepest) - 1);
+  return 4.85f + waves * (1.83f + joins + 2.4f * each) +
          (splits > 1 ? 3.35f + 0.6e-6f * splits * M * float(N) : 0.f);
 }
 
-BlockPlan block_plan(int M, int N, int K, bool aligned) {
-  BlockPlan best{0, 128, 1, 0.f};
-  best.cost = cost_1cta(M, N, K, 128, 1);
+BlockPlan block_plan(int M, int N, int K, bool aligned, int deepest) {
+  BlockPlan best{0, 128, 1, INFINITY, 0};
   const int kb = (K + kScaleBlock - 1) / kScaleBlock;
+  if (deepest == 0 || K <= deepest) best.cost = cost_1cta(M, N, K, 128, 1);
   for (int tn = 16; tn <= 128; tn *= 2) {
     if (tn >= 32 && tn >= 2 * M) break;
     for (int s = 1; s <= 8 && s <= kb; s *= 2) {
+      if (deepest > 0 && (kb + s - 1) / s * kScaleBlock > deepest) continue;
       const float c = cost_1cta(M, N, K, tn, s);
-      if (c < best.cost) best = BlockPlan{0, tn, s, c};
+      if (c < best.cost) best = BlockPlan{0, tn, s, c, deepest};
     }
   }
   if (!aligned) return best;
   for (int s = 1; s <= 8; ++s) {
-    if (!block_2cta_splits_ok(K, s)) continue;
-    const float c = cost_2cta(M, N, K, s);
-    if (c < best.cost) best = BlockPlan{1, 0, s, c};
+    if (!block_2cta_splits_ok(K, s) || (s > 1 && deepest > 0 && block_2cta_depth(K, s) > deepest)) continue;
+    const float c = cost_2cta(M, N, K, s, s > 1 ? 0 : deepest);
+    if (c < best.cost) best = BlockPlan{1, 0, s, c, deepest};
   }
   return best;
 }
 
 // The fused projection and activation on CTA pairs, or the products and a launch that activates and casts
 // (measured at 24 x 9728 x 2560: 25.8 and 17.0 us; 500 x 4096 x 1024: 13.5 and 15.5).
-bool block_glu_fused(int T, int I, int K) {
-  const float fused = cost_2cta(T, 2 * I, K, 1) + 1.f;
-  return fused < block_plan(T, 2 * I, K, true).cost + 2.5f + 2e-6f * T * float(I);
+bool block_glu_fused(int T, int I, int K, int deepest) {
+  const float fused = cost_2cta(T, 2 * I, K, 1, deepest) + 1.f;
+  return fused < block_plan(T, 2 * I, K, true, deepest).cost + 2.5f + 2e-6f * T * float(I);
 }
 
 size_t block_plan_bytes(const BlockPlan& p, int M, int N) {
@@ -570,9 +573,9 @@ int block_gemm(const BlockPlan& p, const BlockMat& A, const BlockMat& B, void* C
   if (p.kernel == 0)
     return block_gemm_1cta(p.tn, p.splits, A, B, C, M, N, K, ldc, out_fp32, accumulate, bias, status, stream);
   if (p.splits == 1)
-    return block_gemm_2cta(1, 0, A, B, C, M, N, K, ldc, out_fp32, accumulate, bias, status, stream);
+    return block_gemm_2cta(1, p.deepest, 0, A, B, C, M, N, K, ldc, out_fp32, accumulate, bias, status, stream);
   const long long stride = 1LL * M * N;
-  const int rc = block_gemm_2cta(p.splits, stride, A, B, ws, M, N, K, N, 1, 0, nullptr, status, stream);
+  const int rc = block_gemm_2cta(p.splits, 0, stride, A, B, ws, M, N, K, N, 1, 0, nullptr, status, stream);
   if (rc) return rc;
   return block_sum(static_cast<const float*>(ws), p.splits, stride, M, N, C, ldc, out_fp32, accumulate, stream);
 }

@@ -14,6 +14,13 @@
 //   warp 0      TMA producer                  warps 2-9    epilogue
 //   warp 1      leader: MMA issuer            warps 10-13  scales
 //
+// DEEP: a tile's contraction is several sums (kDeepestSum says why), each in the accumulator whose turn it is; the
+// epilogue adds them in 128 registers a thread, while the next one is in the making. For these the registers of the other
+// warps go to those of the epilogue, so warpgroups have one role each: warps 4-7 scales, 8-15 epilogue. The gradient of
+// gate and up at 4097 x 2048 x 8192 then is off fp32 sums' by 1.4e-4 of its norm for 1.7e-4, gate and up round on another
+// side than in 64 bits in 4e-5 of the values for 7e-5 (8192 deep: 1.4e-4 for 3.2e-4). Measured in turn without / with,
+// training steps: 4097 x 2048 x 8192 798 / 817 us, 16384 x 2560 x 9728 3754 / 3881.
+//
 // Measured by itself, L2 flushed: 8192 x 4096 x 4096 92 us (2.98 PFLOP/s, the tensor pipe active in 81 % of the cycles),
 // 20960 x 6144 x 4096 334 us (3.16; 360 inside the layer), 16384 x 4096 x 4096 168 (3.27). Bound by the tensor cores where
 // the contraction is deep, and by the power limit over seconds; by the epilogue where it is short (8192 x 8192 x 512 45 us).
@@ -38,7 +45,10 @@ constexpr int kStages = 3;
 constexpr int kGroup = 2;                    // stages that one group of scale words serves
 constexpr int A_BYTES = BM * BK, B_BYTES = BNh * BK, STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = 32 * (2 + kEpiWarps + 4);
+// Warps: with DEEP the scale warps and the epilogue are whole warpgroups (warps 4-7 and 8-15), whose registers differ.
+constexpr int kWarpsPlain = 2 + kEpiWarps + 4, kWarpsDeep = 16;
+constexpr int kRegsLaunch = 128, kRegsFew = 48, kRegsEpi = 208;   // DEEP: of a thread, at launch and from then on
+static_assert(2 * kRegsFew + 2 * kRegsEpi <= 4 * kRegsLaunch && kRegsLaunch * 32 * kWarpsDeep <= 65536, "");
 constexpr int EPI_WORDS = 32 * 33;
 constexpr int kBarBytes = 512;
 constexpr int SMEM_BYTES = kStages * STAGE_BYTES + 1024 + kBarBytes + kEpiWarps * EPI_WORDS * 4;
@@ -56,6 +66,7 @@ struct Block2Args {
   const __nv_bfloat16* bias;
   int a_e5m2, b_e5m2;
   int splits, stages_per_split;
+  int stages_per_sum;                        // DEEP: stages of one sum in tensor memory; else those of a split
   long long split_stride;                    // elements between the outputs of two splits
   int band;                                  // rows of tiles in a band; 0: row by row
   int whole, items;                          // work items: `whole` tiles, then halves of 128 columns
@@ -102,8 +113,18 @@ __device__ __forceinline__ void store_words(void* dst, const uint32_t (&w)[WORDS
   }
 }
 
-template <typename OutT, int GLU>
-__global__ void __launch_bounds__(kThreads, 1)
+// Registers of this warpgroup's threads from here on (all its warps take part).
+template <int REGS>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
+template <typename OutT, int GLU, int DEEP>
+__global__ void __launch_bounds__(32 * (DEEP ? kWarpsDeep : kWarpsPlain), 1)
     gemm_block_2cta_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                            const __grid_constant__ CUtensorMap tmB2, Block2Args g) {
   extern __shared__ uint8_t smem_raw[];
@@ -119,6 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tover + 1);
   float* epi_stage = reinterpret_cast<float*>(smem + kStages * STAGE_BYTES + kBarBytes);
 
+  constexpr int kEpi0 = DEEP ? 8 : 2, kScale0 = DEEP ? 4 : 2 + kEpiWarps;   // first warp of the epilogue, of the scales
   const int warp = warp_index();
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();   // 0 = leader
@@ -182,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   };
   int split, m0, n0, st0, st1;
 
+  if (DEEP && warp < kScale0) fewer_registers<kRegsFew>();
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer
     if (elect_one()) {
@@ -223,51 +246,55 @@ __global__ void __launch_bounds__(kThreads, 1)
       int stage = 0, group = 0, it = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = pair; tile < total && ok; tile += npairs, ++it) {
+      for (int tile = pair; tile < total && ok; tile += npairs) {
         decode(tile, split, m0, n0, st0, st1);
-        const int acc = it & 1;
-        if (!mbar_wait(&tempty[acc], ((it >> 1) & 1) ^ 1u) || (it > 0 && !mbar_wait(tover, (it - 1) & 1))) {
-          report_status(g.status, kStatusTimeoutMma);
-          break;
-        }
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + (acc ? kAcc1 : 0);
         const uint32_t idesc0 = umma_idesc_block(2 * BM, narrow ? BNh : BNp, g.a_e5m2, g.b_e5m2, 0);
         const uint32_t b_half = narrow ? BNh / 2 * 128 : BNh * 128;   // bytes of 128 of depth
-        for (int st = st0; st < st1; ++st) {
-          const int at = (st - st0) % kGroup, slot = group % kSlots;
-          if ((at == 0 && !mbar_wait(&sfull[slot], (group / kSlots) & 1)) || !mbar_wait(&full[stage], phase)) {
+        for (int s0 = st0; s0 < st1 && ok; s0 += g.stages_per_sum, ++it) {
+          const int s1 = min(s0 + g.stages_per_sum, st1), acc = it & 1;
+          if (!mbar_wait(&tempty[acc], ((it >> 1) & 1) ^ 1u) || (it > 0 && !mbar_wait(tover, (it - 1) & 1))) {
             report_status(g.status, kStatusTimeoutMma);
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * STAGE_BYTES), sb = sa + A_BYTES;
-          const uint32_t scales = tmem_base + kScaleCols + 16 * slot;
+          const uint32_t d_tmem = tmem_base + (acc ? kAcc1 : 0);
+          for (int st = s0; st < s1; ++st) {
+            const int at = (st - s0) % kGroup, slot = group % kSlots;
+            if ((at == 0 && !mbar_wait(&sfull[slot], (group / kSlots) & 1)) || !mbar_wait(&full[stage], phase)) {
+              report_status(g.status, kStatusTimeoutMma);
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t sa = smem_u32(smem + stage * STAGE_BYTES), sb = sa + A_BYTES;
+            const uint32_t scales = tmem_base + kScaleCols + 16 * slot;
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            if (k >= 4 && st * BK + kScaleBlock >= g.K) break;   // no second block: nor is there a scale for it
-            const uint32_t sf = uint32_t(2 * at + k / 4);
-            umma2_block(d_tmem, umma_smem_desc(sa + (k / 4) * (BM * 128) + (k % 4) * 32, 16, 1024),
-                        umma_smem_desc(sb + (k / 4) * b_half + (k % 4) * 32, 16, 1024),
-                        idesc0 | (sf << 4) | (sf << 29), scales, scales + 4, st > st0 || k > 0);
+            for (int k = 0; k < 8; ++k) {
+              if (k >= 4 && st * BK + kScaleBlock >= g.K) break;   // no second block: nor is there a scale for it
+              const uint32_t sf = uint32_t(2 * at + k / 4);
+              umma2_block(d_tmem, umma_smem_desc(sa + (k / 4) * (BM * 128) + (k % 4) * 32, 16, 1024),
+                          umma_smem_desc(sb + (k / 4) * b_half + (k % 4) * 32, 16, 1024),
+                          idesc0 | (sf << 4) | (sf << 29), scales, scales + 4, st > s0 || k > 0);
+            }
+            umma2_commit_both(&empty[stage], 1u);
+            if (at == kGroup - 1 || st == s1 - 1) {
+              umma2_commit_both(&sempty[slot], 1u);
+              ++group;
+            }
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
-          umma2_commit_both(&empty[stage], 1u);
-          if (at == kGroup - 1 || st == st1 - 1) {
-            umma2_commit_both(&sempty[slot], 1u);
-            ++group;
-          }
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+          if (ok) umma2_commit_both(&tfull[acc], 1u);
         }
-        if (ok) umma2_commit_both(&tfull[acc], 1u);
       }
     }
     __syncwarp();
-  } else if (warp >= 2 + kEpiWarps) {
+  } else if (warp >= kScale0 && warp < kScale0 + 4) {
     // ------------------------------------------------------------------ scale warps
+    if constexpr (DEEP) fewer_registers<kRegsFew>();
     const uint32_t lanes = uint32_t((warp & 3) * 32) << 16;
     const uint32_t arrive0 = map_to_cta(&sfull[0], 0), arrive1 = map_to_cta(&sfull[1], 0);
     uint32_t wa[4], wb[8];
@@ -318,22 +345,61 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tile += npairs;
     }
-  } else {
-    // ------------------------------------------------------------------ epilogue (warps 2..9)
+  } else if (warp >= kEpi0) {
+    // ------------------------------------------------------------------ epilogue
+    if constexpr (DEEP) more_registers<kRegsEpi>();
     const int q = warp & 3;
-    const int half = (warp - 2) >> 2;
+    const int half = (warp - kEpi0) >> 2;
     const uint32_t tempty0 = map_to_cta(&tempty[0], 0), tempty1 = map_to_cta(&tempty[1], 0);
     const uint32_t over = map_to_cta(tover, 0);
-    uint8_t* sblk = reinterpret_cast<uint8_t*>(epi_stage + (warp - 2) * EPI_WORDS);
+    uint8_t* sblk = reinterpret_cast<uint8_t*>(epi_stage + (warp - kEpi0) * EPI_WORDS);
     int it = 0;
     bool ok = true;
     for (int tile = pair; tile < total; tile += npairs, ++it) {
       decode(tile, split, m0, n0, st0, st1);
-      const int acc = it & 1;
-      if (ok && !__all_sync(0xffffffffu, mbar_wait(&tfull[acc], (it >> 1) & 1))) {
-        report_status(g.status, kStatusTimeoutEpilogue);
-        ok = false;
+      // the sum that is next in tensor memory
+      auto arrived = [&] {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait(&tfull[it & 1], (it >> 1) & 1));
+        if (!ok) report_status(g.status, kStatusTimeoutEpilogue);
+        return ok;
+      };
+      // DEEP: all sums of the tile but the last, 32 columns a group, added in their order
+      float before[DEEP ? 4 : 1][32];
+      if constexpr (DEEP) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 32; ++j) before[i][j] = 0.f;
+        for (int s0 = st0; ok && s0 + g.stages_per_sum < st1; s0 += g.stages_per_sum, ++it) {
+          if (!arrived()) break;
+          tc_fence_after();
+          const int acc = it & 1;
+          const uint32_t src = tmem_base + (uint32_t(q * 32) << 16) + (acc ? kAcc1 : 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // (the groups of the tile's end below, in the same order)
+            const int c = GLU ? 2 * half + ((i / 2 - half) & 1) + (i & 1) * (BNh / 32)
+                              : (narrow ? 2 : 4) * half + ((i - half) & (narrow ? 1 : 3));
+            if (GLU || !narrow || i < 2) {
+              uint32_t r[32];
+              tmem_ld_32x32b_x32(src + c * 32, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) before[i][j] += __uint_as_float(r[j]);
+            }
+            if (i == (GLU ? 1 : 0) && half != acc) {   // gate and up, or the one, of the columns that are shared
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_remote(over);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(acc ? tempty1 : tempty0);
+        }
       }
+      const int acc = it & 1;
+      if (ok) arrived();
       if (!ok) {   // (the two warps of a row meet at a barrier for each tile, whatever either has waited for)
         if (GLU) asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
         continue;
@@ -343,7 +409,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int row = m0 + q * 32 + lane;
       // the columns that the other accumulator shares: this one's last (acc 0) or first 32
       const bool shared_here = half != acc;
-      const int rot = acc == 0 && half == 1 ? -1 : 0;   // start with the last chunk of the half
+      // start with the last chunk of the half (DEEP: whichever accumulator it is, so that sums stay where they are)
+      const int rot = (DEEP || acc == 0) && half == 1 ? -1 : 0;
       if constexpr (GLU) {
         uint32_t h[2][16];
         uint32_t top = 0u;
@@ -358,6 +425,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(over);
+          }
+          if constexpr (DEEP) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              rg[j] = __float_as_uint(before[2 * i][j] + __uint_as_float(rg[j]));
+              ru[j] = __float_as_uint(before[2 * i + 1][j] + __uint_as_float(ru[j]));
+            }
           }
           uint32_t w[2][16];   // gate, up
 #pragma unroll
@@ -416,8 +490,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       } else {
         OutT* Cout = reinterpret_cast<OutT*>(g.C) + split * g.split_stride;
         const int chunks = narrow ? 2 : 4;   // of 32 columns, a half of the warps
-#pragma unroll 1
-        for (int i = 0; i < chunks; ++i) {
+#pragma unroll(DEEP ? 4 : 1)
+        for (int i = 0; i < (DEEP ? 4 : chunks); ++i) {
+          if (DEEP && i >= chunks) continue;
           const int c = chunks * half + ((i + rot) & (chunks - 1));
           uint32_t r[32];
           tmem_ld_32x32b_x32(src0 + c * 32, r);
@@ -426,6 +501,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_remote(over);
+          }
+          if constexpr (DEEP) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r[j] = __float_as_uint(before[i][j] + __uint_as_float(r[j]));
           }
           const int col0 = n0 + c * 32;
           if (g.bias != nullptr) {
@@ -479,16 +558,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 constexpr int kMaxDevices = 64;
 int g_pairs[kMaxDevices];   // CTA pairs resident at once; 0: not asked yet
 
-template <typename OutT, int GLU>
+template <typename OutT, int GLU, int DEEP>
 int launch_2cta(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmB2, Block2Args& g,
                 long long total, cudaStream_t stream) {
-  auto kern = gemm_block_2cta_kernel<OutT, GLU>;
+  auto kern = gemm_block_2cta_kernel<OutT, GLU, DEEP>;
+  constexpr int kThreads = 32 * (DEEP ? kWarpsDeep : kWarpsPlain);
   static bool configured[kMaxDevices] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return -10;
   if (!configured[dev]) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess)
       return -10;
+    cudaFuncAttributes is{};
+    // (warps that ask for more than the block was launched with would wait for good)
+    if (DEEP && (cudaFuncGetAttributes(&is, kern) != cudaSuccess || is.numRegs != kRegsLaunch)) return -12;
     configured[dev] = true;
   }
   if (g_pairs[dev] == 0) {
@@ -531,6 +614,9 @@ int stages_of_split(int K, int splits) {
   const int stages = (K + BK - 1) / BK;
   return ((stages + splits - 1) / splits + kGroup - 1) / kGroup * kGroup;   // whole groups of scale words
 }
+// Stages of one sum: equal parts of the contraction, of `deepest` at most.
+int stages_of_sum(int K, int deepest) { return stages_of_split(K, block_2cta_sums(K, deepest)); }
+static_assert(kDeepestSum % (kGroup * BK) == 0, "");
 
 }  // namespace
 
@@ -539,11 +625,17 @@ bool block_2cta_splits_ok(int K, int splits) {
   return (stages + each - 1) / each == splits;
 }
 
+int block_2cta_sums(int K, int deepest) { return deepest > 0 ? (K + deepest - 1) / deepest : 1; }
+int block_2cta_depth(int K, int splits) { return stages_of_split(K, splits) * BK; }
+
 // N a multiple of 8, C 16-byte aligned, ldc a multiple of 8. splits > 1 (fp32): split s of the contraction writes its
-// own sums to C + s * split_stride.
-int block_gemm_2cta(int splits, long long split_stride, const BlockMat& A, const BlockMat& B, void* C, int M,
+// own sums to C + s * split_stride. deepest > 0 (bf16 without bias, splits = 1): sums of tensor memory are that deep at
+// most, and added in registers.
+int block_gemm_2cta(int splits, int deepest, long long split_stride, const BlockMat& A, const BlockMat& B, void* C, int M,
                     int N, int K, long long ldc, int out_fp32, int accumulate, const void* bias, int* status,
                     cudaStream_t stream) {
+  const bool deep = block_2cta_sums(K, deepest) > 1;
+  if (deep && (splits > 1 || out_fp32 || bias != nullptr || deepest % (kGroup * BK))) return -5;
   if ((N & 7) || (ldc & 7) || (reinterpret_cast<uintptr_t>(C) & 15)) return -5;
   if (splits > 1 && (!out_fp32 || accumulate || bias != nullptr)) return -5;
   if (splits < 1 || !block_2cta_splits_ok(K, splits)) return -5;
@@ -572,20 +664,24 @@ int block_gemm_2cta(int splits, long long split_stride, const BlockMat& A, const
   g.b_e5m2 = B.e5m2 ? 1 : 0;
   g.splits = splits;
   g.stages_per_split = stages_of_split(K, splits);
+  g.stages_per_sum = deep ? stages_of_sum(K, deepest) : g.stages_per_split;
   g.split_stride = splits > 1 ? split_stride : 0;
   if (g.split_stride & 7) g.wide = 0;
   g.band = band_of(tiles_n, 1LL * N * K);
   g.status = status;
   const long long total = 1LL * tiles_m * tiles_n * splits;
   if (total > 0x7fff0000LL) return -3;   // (tiles are counted in steps of the grid)
-  return out_fp32 ? launch_2cta<float, 0>(tmA, tmB, tmBh, g, total, stream)
-                  : launch_2cta<__nv_bfloat16, 0>(tmA, tmB, tmBh, g, total, stream);
+  if (out_fp32) return launch_2cta<float, 0, 0>(tmA, tmB, tmBh, g, total, stream);
+  return deep ? launch_2cta<__nv_bfloat16, 0, 1>(tmA, tmB, tmBh, g, total, stream)
+              : launch_2cta<__nv_bfloat16, 0, 0>(tmA, tmB, tmBh, g, total, stream);
 }
 
 // gate and up weights [I, K], I a multiple of 128, with a common row stride and scale words of common groups. Both
-// products, rounded to bf16, also go to gate and up (rows ld_gu elements apart) unless those are null.
-int block_gemm_glu(int kind, const BlockMat& A, const BlockMat& Wg, const BlockMat& Wu, int M, int I, int K,
+// products, rounded to bf16, also go to gate and up (rows ld_gu elements apart) unless those are null. deepest: as above.
+int block_gemm_glu(int kind, int deepest, const BlockMat& A, const BlockMat& Wg, const BlockMat& Wu, int M, int I, int K,
                    void* gate, void* up, long long ld_gu, const BlockMat& h, int* status, cudaStream_t stream) {
+  const bool deep = block_2cta_sums(K, deepest) > 1;
+  if (deep && deepest % (kGroup * BK)) return -5;
   if ((I % kScaleBlock) || (ld_gu & 7) || (gate == nullptr) != (up == nullptr) || Wg.rows_s != Wu.rows_s) return -3;
   CUtensorMap tmA, tmG, tmU;
   int rc = make_tmap_2d(&tmA, A.data, 1, (uint64_t)K, (uint64_t)M, (uint64_t)A.ld, 128, BM, true);
@@ -613,6 +709,7 @@ int block_gemm_glu(int kind, const BlockMat& A, const BlockMat& Wg, const BlockM
   g.b_e5m2 = Wg.e5m2 ? 1 : 0;
   g.splits = 1;
   g.stages_per_split = stages_of_split(K, 1);
+  g.stages_per_sum = deep ? stages_of_sum(K, deepest) : g.stages_per_split;
   g.band = band_of(tiles_n, 2LL * I * K);
   g.h = h.data;
   g.ldh = h.ld;
@@ -621,8 +718,11 @@ int block_gemm_glu(int kind, const BlockMat& A, const BlockMat& Wg, const BlockM
   g.status = status;
   const long long total = 1LL * tiles_m * tiles_n;
   if (total > 0x7fff0000LL) return -3;   // (tiles are counted in steps of the grid)
-  return kind == kSwiglu ? launch_2cta<__nv_bfloat16, 1 + kSwiglu>(tmA, tmG, tmU, g, total, stream)
-                         : launch_2cta<__nv_bfloat16, 1 + kGeglu>(tmA, tmG, tmU, g, total, stream);
+  if (deep)
+    return kind == kSwiglu ? launch_2cta<__nv_bfloat16, 1 + kSwiglu, 1>(tmA, tmG, tmU, g, total, stream)
+                           : launch_2cta<__nv_bfloat16, 1 + kGeglu, 1>(tmA, tmG, tmU, g, total, stream);
+  return kind == kSwiglu ? launch_2cta<__nv_bfloat16, 1 + kSwiglu, 0>(tmA, tmG, tmU, g, total, stream)
+                         : launch_2cta<__nv_bfloat16, 1 + kGeglu, 0>(tmA, tmG, tmU, g, total, stream);
 }
 
 }  // namespace lb

@@ -489,3 +489,48 @@ def test_a_run_through_models_training_and_encoding():
     assert sum(isinstance(m, Fp8KeptLinear) for m in model.modules()) == 2 * 6
     assert torch.nn.functional.cosine_similarity(got, want, dim=-1).min().item() > 0.97
     nv.check_status()
+
+
+# ------------------------------------------------------------------------------------------------
+# Sums
+# ------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("T,H,I", [(1024, 8192, 1024), (1000, 2560, 2048), (2600, 2048, 1024), (64, 4096, 4096)])
+@pytest.mark.parametrize("kind", ["swiglu", "geglu"])
+def test_what_a_step_rounds_twice_is_summed_as_in_32_bits(T, H, I, kind):
+    """Gate and up products are rounded to bf16 and, as gradients, to 8 bits, where a sum on the wrong side of a border
+    moves a value by 2^-4 of itself. So no more of them may fall on another side than 64 bits put them than of sums in
+    plain fp32: half as many again, and six standard deviations of such a count."""
+    x, w, wd = _rand(T, H, spread=0.5), _rand(2 * I, H, seed=1, spread=0.3) * H ** -0.5, _rand(H, I, seed=2, spread=0.3)
+    y = fb.gated_mlp_fp8_block(x, w.requires_grad_(), None, wd, kind)
+    nv.check_status()
+    saved = y.grad_fn.saved_tensors[-1]                   # gate and up products come first in it
+    gu = saved[:4 * T * I].view(torch.bfloat16).view(T, 2 * I)
+    xv, wv = _value(x, 1, 128), _value(w, 128, 128)
+    exact = (xv @ wv.t()).to(torch.float32).to(torch.bfloat16)
+    plain = int(((xv.float() @ wv.float().t()).to(torch.bfloat16) != exact).sum())
+    own = int((gu != exact).sum())
+    assert own <= 1.5 * plain + 6 * max(plain, 1) ** 0.5, (own, plain)
+
+
+@pytest.mark.parametrize("T", [40, 3000])
+def test_gradients_of_a_deep_step_against_64_bits(T):
+    """The gradient of gate and up, in an fp32 accumulator, beside the formula's in 64 bits: no further off than where the
+    sums in front of the two roundings are plain fp32 ones, twice that and what its own sums add."""
+    H, I = 8192, 512
+    x, dy = _rand(T, H, spread=0.5), _rand(T, H, seed=1, spread=1.0)
+    w, wd = _rand(2 * I, H, seed=2, spread=0.3) * H ** -0.5, _rand(H, I, seed=3, spread=0.3) * I ** -0.5
+    w.requires_grad_()
+    w.main_grad = torch.zeros(2 * I, H, device="cuda")
+    fb.gated_mlp_fp8_block(x, w, None, wd).backward(dy)
+    nv.check_status()
+
+    def gradient(dtype):
+        xv, wv, dv, yv = (_value(*a).to(dtype) for a in ((x, 1, 128), (w, 128, 128), (wd, 128, 128), (dy, 1, 128)))
+        gu, dh = (xv @ wv.t()).to(torch.bfloat16).to(dtype), (yv @ dv).to(torch.bfloat16).to(dtype)
+        g, u = gu.chunk(2, dim=1)
+        s = 1 / (1 + torch.exp(-g))
+        d = torch.cat([dh * u * s * (1 + g * (1 - s)), dh * g * s], dim=1).to(torch.bfloat16)
+        return _value(d, 128, 1).t() @ _value(x, 128, 1)
+
+    want = gradient(torch.float64)
+    assert _off(w.main_grad, want) <= 2 * _off(gradient(torch.float32), want) + (T // 32 + 3) * 2.0 ** -22
