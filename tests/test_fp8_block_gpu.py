@@ -534,3 +534,51 @@ def test_gradients_of_a_deep_step_against_64_bits(T):
 
     want = gradient(torch.float64)
     assert _off(w.main_grad, want) <= 2 * _off(gradient(torch.float32), want) + (T // 32 + 3) * 2.0 ** -22
+
+
+@pytest.mark.parametrize("kind", ["swiglu", "geglu"])
+@pytest.mark.parametrize("T", [24, None])
+def test_activation_and_derivative_of_every_gate(kind, T):
+    """Gates of every bf16 value from 2^-40 to 2^20 (the upper and the lower half of the bits lie in blocks of their own,
+    so nothing is rounded on the way to the product), up projections of 1. y is 2^67 times act(g) in 8 bits, the gradient
+    of x's first column 128 times the derivative."""
+    bits = torch.arange((127 - 40) << 7, (127 + 20) << 7, device="cuda", dtype=torch.int32)
+    g = (torch.cat([bits, bits | 0x8000]) << 16).view(torch.float32)
+    if T is not None:       # gates whose sigmoid is far from 0 and 1, and at its lower end
+        near = torch.tensor([-88.5, -88, -87.5, -87, -60, -17, -5, -3, -1, -0.5, 0.5, 3], device="cuda")
+        g = torch.cat([near, torch.linspace(-4, 4, T - 12, device="cuda").to(torch.bfloat16).float()])
+    low = (g.view(torch.int32) & 0x000F0000) != 0
+    top = (g.view(torch.int32) & ~0x000FFFFF).view(torch.float32)
+    x = torch.zeros(len(g), 384, device="cuda")
+    x[:, 0], x[:, 128], x[:, 256] = top, torch.where(low, g - top, torch.zeros_like(g)), 1
+    w = torch.zeros(256, 384, device="cuda")
+    w[:128, 0] = w[:128, 128] = w[128:, 256] = 1
+    wd, dy = torch.zeros(384, 128, device="cuda"), torch.zeros(len(g), 384, device="cuda")
+    wd[0], dy[:, 0] = 2.0 ** 60, 2.0 ** -60
+    x, w, wd, dy = (t.to(torch.bfloat16).requires_grad_() for t in (x, w, wd, dy))
+    y = fb.gated_mlp_fp8_block(x, w, None, wd, kind)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    nv.check_status()
+    if kind == "swiglu":
+        s = 1 / (1 + torch.exp(-g))
+        a, da = g * s, s * (1 + g * (1 - s))
+        v = g.double()
+        s = 1 / (1 + torch.exp(-v))
+        exact = v * s, s * (1 + v * (1 - s))
+    else:
+        c, k = 0.7978845608028654, 0.044715
+        t = torch.tanh(c * (g + k * g * g * g))
+        a, da = 0.5 * g * (1 + t), 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * c * (1 + 3 * k * g * g)
+        exact = None
+    for i, (got, plain) in enumerate(((y[:, 0].double() * 2.0 ** -67, a), (dx[:, 0].double() / 128, da))):
+        want = _value(plain.to(torch.bfloat16).view(-1, 1).expand(-1, 8), 1, 128)[:, 0]
+        # the formula in 32 bits, operation by operation, as far as the sigmoid is not 0 (below -87.3). Gates below -1, one in
+        # 16 here, have it off by up to 2^-24 |g| of itself, 2^-18: between bf16 values 2^-8 apart one in 2^9 then falls
+        # to another side, and of those one in 2^4 in 8 bits, which have 16 steps of bf16 to one of their own.
+        some = g >= -87.25
+        assert int((got != want)[some].sum()) <= 3 + len(g) * 2.0 ** -17, int((got != want)[some].sum())
+        assert (got[~some].abs() <= 2.0 ** -116).all()
+        if exact is not None:
+            e, v = exact[i][some], got[some]
+            # 1 - s and 1 + g (1 - s) cancel next to the derivative's zero: an absolute error there
+            assert ((v - e).abs() <= (2.0 ** -4 + 2.0 ** -8) * e.abs() + 2.0 ** -20 * (e.abs() > 2.0 ** -30)).all()
