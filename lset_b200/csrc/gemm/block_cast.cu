@@ -410,11 +410,12 @@ __global__ void __launch_bounds__(512, 2)
   }
 }
 
-// out [rows, cols] = (out +) sums of P matrices, part p at p * stride, each value in the order of p.
+// out [rows, cols] = (out +) sums of P matrices, part p at p * stride, each value in the order of p, and bias [cols] behind
+// them (null: none).
 template <typename OutT>
 __global__ void __launch_bounds__(256)
     block_sum_kernel(const float* __restrict__ part, int P, long long stride, int rows, int cols, OutT* out,
-                     long long ldo, int accumulate) {
+                     long long ldo, int accumulate, const bf16* __restrict__ bias) {
   pdl_wait();
   pdl_trigger();
   const int vecs = cols / 4;
@@ -427,6 +428,10 @@ __global__ void __launch_bounds__(256)
     for (int p = 0; p < P; ++p) {
       const float4 v = *reinterpret_cast<const float4*>(part + p * stride + 4 * i);
       s = make_float4(s.x + v.x, s.y + v.y, s.z + v.z, s.w + v.w);
+    }
+    if (bias != nullptr) {   // (at any multiple of 2 bytes)
+      s = make_float4(s.x + __bfloat162float(bias[c]), s.y + __bfloat162float(bias[c + 1]),
+                      s.z + __bfloat162float(bias[c + 2]), s.w + __bfloat162float(bias[c + 3]));
     }
     OutT* o = out + r * ldo + c;
     if constexpr (sizeof(OutT) == 2) {
@@ -575,16 +580,17 @@ int block_glu_bwd(int kind, const void* dh, long long ld_dh, const void* gate, c
 
 // cols a multiple of 4; part, stride and out 16-byte aligned (out: 8 bytes in bf16).
 int block_sum(const float* part, int P, long long stride, int rows, int cols, void* out, long long ldo,
-              int out_fp32, int accumulate, cudaStream_t stream) {
+              int out_fp32, int accumulate, const void* bias, cudaStream_t stream) {
   if (rows <= 0 || cols <= 0) return 0;
   if ((cols & 3) || (stride & 3) || (ldo & 3) || (accumulate && !out_fp32)) return -3;
+  const bf16* b = static_cast<const bf16*>(bias);
   const long long n = 1LL * rows * (cols / 4);
   const unsigned grid = unsigned(n > 148LL * 8 * 256 ? 148 * 8 : (n + 255) / 256);
   const bool pdl = pdl_enabled(4LL * P * rows * cols);
   return out_fp32 ? launch_pdl(block_sum_kernel<float>, dim3(grid), dim3(256), 0, stream, pdl, 1, part, P, stride,
-                               rows, cols, static_cast<float*>(out), ldo, accumulate)
+                               rows, cols, static_cast<float*>(out), ldo, accumulate, b)
                   : launch_pdl(block_sum_kernel<bf16>, dim3(grid), dim3(256), 0, stream, pdl, 1, part, P, stride,
-                               rows, cols, static_cast<bf16*>(out), ldo, 0);
+                               rows, cols, static_cast<bf16*>(out), ldo, 0, b);
 }
 
 }  // namespace lb

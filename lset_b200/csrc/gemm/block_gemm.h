@@ -86,8 +86,8 @@ int block_glu_fwd(int kind, const void* gate, const void* up, long long ld, int 
 int block_glu_bwd(int kind, const void* dh, long long ld_dh, const void* gate, const void* up, long long ld,
                   int T, int I, const BlockMat& d, const BlockMat& d_t, const BlockMat& h_t,
                   cudaStream_t stream);
-// out [rows, cols] (bf16 or fp32, rows ldo apart) = or += the sum of P matrices [rows, cols] of fp32, in order.
+// out [rows, cols] (bf16 or fp32, rows ldo apart) = or += the sum of P matrices [rows, cols] of fp32, in order, + bias.
 int block_sum(const float* part, int P, long long stride, int rows, int cols, void* out, long long ldo,
-              int out_fp32, int accumulate, cudaStream_t stream);
+              int out_fp32, int accumulate, const void* bias, cudaStream_t stream);
 
 }  // namespace lb

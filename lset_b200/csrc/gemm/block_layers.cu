@@ -230,7 +230,7 @@ extern "C" int lb_linear_block_bwd(const void* dy, long long lddy, int T, int K,
   if (need & 1) c.product(s.dy, s.w_t, Out{dx, dx_mode}, T, K, N, K);
   if (need & 2) c.product(s.dy_t, s.x_t, Out{dw, dw_mode}, N, K, T, K);
   if (need & 4)
-    c.run([&] { return block_sum(s.colsum, (T + 127) / 128, N, 1, N, db, N, db_mode, 0, c.stream); });
+    c.run([&] { return block_sum(s.colsum, (T + 127) / 128, N, 1, N, db, N, db_mode, 0, nullptr, c.stream); });
   return c.rc;
 }
 

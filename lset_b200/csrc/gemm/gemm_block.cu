@@ -577,7 +577,8 @@ int block_gemm(const BlockPlan& p, const BlockMat& A, const BlockMat& B, void* C
   const long long stride = 1LL * M * N;
   const int rc = block_gemm_2cta(p.splits, 0, stride, A, B, ws, M, N, K, N, 1, 0, nullptr, status, stream);
   if (rc) return rc;
-  return block_sum(static_cast<const float*>(ws), p.splits, stride, M, N, C, ldc, out_fp32, accumulate, stream);
+  return block_sum(static_cast<const float*>(ws), p.splits, stride, M, N, C, ldc, out_fp32, accumulate, bias,
+                   stream);
 }
 
 }  // namespace lb

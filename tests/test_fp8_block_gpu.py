@@ -582,3 +582,36 @@ def test_activation_and_derivative_of_every_gate(kind, T):
             e, v = exact[i][some], got[some]
             # 1 - s and 1 + g (1 - s) cancel next to the derivative's zero: an absolute error there
             assert ((v - e).abs() <= (2.0 ** -4 + 2.0 ** -8) * e.abs() + 2.0 ** -20 * (e.abs() > 2.0 ** -30)).all()
+
+
+# contractions that CTA pairs split over several products in fp32 (few tiles, great depth), ragged ones among them
+SPLIT = [(333, 1024, 8192), (300, 1016, 8328), (1000, 512, 9728), (700, 776, 16392), (1024, 1024, 16384)]
+
+
+@pytest.mark.parametrize("M,N,K", SPLIT)
+def test_split_products_with_bias(M, N, K):
+    assert fb._product_bytes(M, N, K, N) >= 2 * 4 * M * N
+    a, _ = fb.quantize_fp8_block(_rand(M, K, spread=1.0))
+    b, _ = fb.quantize_fp8_block(_rand(N, K, seed=1, spread=1.0), tile=True)
+    wide = _rand(N + 1, spread=0.5) * K ** 0.5
+    for bias in (wide[:N], wide[1:]):      # the second at no multiple of 4 bytes
+        for dt in (torch.bfloat16, torch.float32):
+            _check_product(fb.matmul_fp8_block(a, b, bias=bias, out_dtype=dt), a, b, bias)
+    nv.check_status()
+
+
+@pytest.mark.parametrize("T,N,K", [(333, 1024, 8192), (1000, 512, 9728)])
+def test_split_layers_with_bias(T, N, K):
+    x, w, b = _rand(T, K, spread=1.0), _rand(N, K, seed=1, spread=0.5), _rand(N, seed=2, spread=0.5) * K ** 0.5
+    xq, _ = fb.quantize_fp8_block(x)
+    wq, _ = fb.quantize_fp8_block(w, tile=True)
+    x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+    y = fb.linear_fp8_block(x, w, b)
+    _check_product(y.detach(), xq, wq, b.detach())
+    dy = _rand(T, N, seed=3)
+    (db,) = torch.autograd.grad(y, b, dy)
+    assert ((db.double() - dy.double().sum(0)).abs()
+            <= 2.0 ** -8 * dy.double().sum(0).abs() + T * 2.0 ** -24 * dy.double().abs().sum(0)).all()
+    with torch.no_grad():
+        assert torch.equal(fb.linear_fp8_block(x, wq, b), y)
+    nv.check_status()
