@@ -415,3 +415,59 @@ def test_evaluation_of_a_model_with_the_recipe_keeps_8_bit_weights(monkeypatch):
         cfg.fp8.enabled, cfg.fp8.recipe = enabled, recipe
         run_eval(cfg)
     assert seen == [True, False, False]
+
+
+# ------------------------------------------------------------------------------------------------
+# Whose memory a matrix is
+# ------------------------------------------------------------------------------------------------
+def _copies(q, tmp_path):
+    import copy
+    import pickle
+
+    torch.save(q, tmp_path / "q.pt")
+    return {"deepcopy": copy.deepcopy(q), "pickle": pickle.loads(pickle.dumps(q)),
+            "save": torch.load(tmp_path / "q.pt", weights_only=False)}
+
+
+@pytest.mark.parametrize("rows,cols,e5m2", [(40, 640, False), (1, 136, True), (0, 64, False)])
+def test_copies_are_on_memory_of_their_own(rows, cols, e5m2, tmp_path):
+    import copy
+
+    q, _ = fb.quantize_fp8_block(torch.randn(rows, cols), e5m2=e5m2)
+    values = q.dequantize()
+    for name, c in _copies(q, tmp_path).items():
+        assert type(c) is fb.Fp8BlockTensor and c.shape == q.shape and c.e5m2 == q.e5m2, name
+        assert c._where == (c.data.data_ptr(), q._where[1], c.scales.data_ptr(), q._where[3]), name
+        assert rows == 0 or (c._where[0] != q._where[0] and c._where[2] != q._where[2]), name
+    same = copy.copy(q)
+    assert same.data is q.data and same._where == q._where
+    copies = _copies(q, tmp_path)
+    q.data.zero_()
+    assert all(torch.equal(c.dequantize(), values) for c in copies.values())
+
+
+def test_parts_of_a_matrix_copy_with_their_strides(tmp_path):
+    b, _ = fb.quantize_fp8_block(torch.randn(384, 640), tile=True)
+    part = fb.Fp8BlockTensor(b.data[128:256, :512], 512, b.scales[:1, 128:256])
+    for c in _copies(part, tmp_path).values():
+        assert c._where[1] == c.data.stride(0) and torch.equal(c.dequantize(), part.dequantize())
+
+
+def test_exchanged_memory_is_looked_at_again():
+    q, _ = fb.quantize_fp8_block(torch.randn(40, 640))
+    other, _ = fb.quantize_fp8_block(torch.randn(40, 640))
+    q.data.data, q.scales.data = other.data, other.scales
+    assert q._where == (other.data.data_ptr(), 640, other.scales.data_ptr(), 40)
+    q.data.data = torch.zeros(40, 656, dtype=torch.uint8)
+    assert q._where == (q.data.data_ptr(), 656, other.scales.data_ptr(), 40)
+    q.scales.data = torch.zeros(2, 39, 4, dtype=torch.uint8)      # a row less
+    with pytest.raises(ValueError, match="belong together"):
+        q._where
+    q.scales.data = other.scales
+    q.data.data = torch.zeros(656, 40, dtype=torch.uint8).t()
+    with pytest.raises(ValueError, match="next to one another"):
+        q._where
+    q.data.data = other.data
+    q.data.untyped_storage().resize_(0)
+    with pytest.raises(ValueError, match="released"):
+        q._where

@@ -615,3 +615,23 @@ def test_split_layers_with_bias(T, N, K):
     with torch.no_grad():
         assert torch.equal(fb.linear_fp8_block(x, wq, b), y)
     nv.check_status()
+
+
+def test_copies_of_kept_weights_are_on_memory_of_their_own():
+    import copy
+    import pickle
+
+    x = _rand(20, 512, spread=0.5)
+    q, _ = fb.quantize_fp8_block(_rand(256, 512, seed=1, spread=0.3), tile=True)
+    with torch.no_grad():
+        want = fb.linear_fp8_block(x, q)
+        for c in (copy.deepcopy(q), pickle.loads(pickle.dumps(q))):
+            q.data.zero_(), q.scales.fill_(127)
+            assert c.data.is_cuda and torch.equal(fb.linear_fp8_block(x, c), want)
+            q.data.copy_(c.data), q.scales.copy_(c.scales)
+        other, _ = fb.quantize_fp8_block(_rand(256, 512, seed=2, spread=0.3), tile=True)
+        q.data.data, q.scales.data = other.data, other.scales
+        assert torch.equal(fb.linear_fp8_block(x, q), fb.linear_fp8_block(x, other))
+        q.scales.data = torch.zeros(1025, dtype=torch.uint8, device="cuda")[1:].view(1, 256, 4)
+        with pytest.raises(ValueError, match="multiples of"):
+            fb.linear_fp8_block(x, q)
