@@ -204,6 +204,7 @@ __device__ __forceinline__ bool cast_rows(const BlockArgs& g, uint8_t* smem, uin
       fence_proxy_async_smem();
       asm volatile("bar.sync 1, 128;" ::: "memory");
       int at = first;
+      tc_fence_after();   // the products of these stages' last blocks are behind (`empty`)
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         if (base + half * kBatch + i >= kb1) break;
@@ -350,6 +351,7 @@ __global__ void __launch_bounds__(kThreads1, 2)
         const int slot = i % kSlots;
         // (all lanes take part in the store, and may see a bounded wait end differently)
         if (!__all_sync(0xffffffffu, mbar_wait(&sempty[slot], ((i / kSlots) & 1) ^ 1u))) return false;
+        tc_fence_after();   // the products that read the slot are behind
         if (CAST)
           tmem_st_32x32b_x4(tmem + lanes + F::kAcc + 8 * slot, w[0], w[1], w[2], w[3]);
         else

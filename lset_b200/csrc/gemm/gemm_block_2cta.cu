@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(32 * (DEEP ? kWarpsDeep : kWarpsPlain), 1)
           const uint32_t d_tmem = tmem_base + (acc ? kAcc1 : 0);
           for (int st = s0; st < s1; ++st) {
             const int at = (st - s0) % kGroup, slot = group % kSlots;
-            if ((at == 0 && !mbar_wait(&sfull[slot], (group / kSlots) & 1)) || !mbar_wait(&full[stage], phase)) {
+            if ((at == 0 && !mbar_wait_cluster(&sfull[slot], (group / kSlots) & 1)) || !mbar_wait(&full[stage], phase)) {
               report_status(g.status, kStatusTimeoutMma);
               ok = false;
               break;
@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(32 * (DEEP ? kWarpsDeep : kWarpsPlain), 1)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(slot ? arrive1 : arrive0);
+        if (lane == 0) mbar_arrive_cluster(slot ? arrive1 : arrive0);
         if (w < last) {
           fetch(w + 1);
         } else if (tile + npairs < total) {

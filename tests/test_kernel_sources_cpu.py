@@ -63,3 +63,34 @@ def test_every_thread_of_the_small_gemm_waits_before_it_stores():
     text = next(t for t in TEXTS.values() if "void cluster_sync_()" in t)
     barrier = text[text.index("void cluster_sync_()"):]
     assert barrier.index("__syncwarp();") < barrier.index("barrier.cluster.arrive")
+
+
+def _source(name):
+    return next(text for p, text in TEXTS.items() if p.name == name)
+
+
+def test_scales_are_written_behind_the_products_that_read_them():
+    """A slot of scale words in tensor memory is written again once the products that read it are done: between the wait
+    that says so and the store there is a fence."""
+    for name, stores in (("gemm_block.cu", 3), ("gemm_block_2cta.cu", 2)):
+        text = _source(name)
+        found = [m.start() for m in re.finditer(r"tmem_st_32x32b_x\d\(tmem|tmem_st_32x32b_x\d\(dst|\"tcgen05\.st\.", text)]
+        assert len(found) == stores, name
+        for at in found:
+            wait = max(text.rfind("mbar_wait(&sempty[", 0, at), text.rfind("mbar_wait(&empty[", 0, at))
+            assert "tc_fence_after();" in text[wait:at], (name, text[at:at + 80])
+
+
+def test_scales_of_the_second_cta_are_handed_over_across_the_cluster():
+    """Tensor memory that a warp of the one CTA has written is read by products that a thread of the other issues: the
+    arrival and the wait are at the scope of both, between the fences of tensor memory."""
+    text = _source("gemm_block_2cta.cu")
+    scales = text[text.index("tmem_st_32x32b_x8(dst"):text.index("if (w < last) {")]
+    assert re.findall(r"tmem_st_wait|tc_fence_before|mbar_arrive\w*", scales) == ["tmem_st_wait", "tc_fence_before",
+                                                                               "mbar_arrive_cluster"]
+    (wait,) = re.finditer(r"mbar_wait\w*\(&sfull", text)
+    assert wait.group() == "mbar_wait_cluster(&sfull"
+    assert "tc_fence_after();" in text[wait.start():text.index("umma2_block(d_tmem")]
+    pair = _source("pair.cuh")
+    assert "mbarrier.arrive.relaxed.cluster.shared::cluster.b64" in pair
+    assert "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64" in pair
