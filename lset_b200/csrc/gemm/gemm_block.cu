@@ -506,12 +506,13 @@ int block_gemm_cast(const BlockPlan& p, const void* x, long long ldx, const Bloc
                     : launch_block<32, 1>(tmP, tmP, g, tiles, p.splits, stream);
 }
 
-// Modelled time (us) of a product, fitted to 887 runs of 116 sizes (rows 1 to 6144, columns 768 to 19456, depths 257
-// to 9728, every tile and split that fits, with what a launch costs in a CUDA graph): off by 17 % in the mean for the
-// one-CTA kernel, by 6 % for the pairs; the variant it chooses takes 1.5 % longer than the best in the mean and 19 % at
-// most. Measured at what the choice turns on: 128 x 2304 x 768 5.0 us in tiles of 16, 7.9 on pairs; 128 x 19456 x 2560
-// 17.8 in tiles of 128, 36.9 of 16; 12 x 2560 x 9728 10.1 split four ways, 19.4 whole; 1000 x 4096 x 2560 13.7 on
-// pairs, 16.2 in tiles of 128; 768 x 1152 x 8191 17.3 on pairs split four ways, 25 whole.
+// Modelled time (us) of a product, beside 1431 runs of 173 sizes (rows 1 to 6144, columns 256 to 19456, depths 256 to
+// 9728, every tile and split that fits, with what a launch costs in a CUDA graph): off by 13 % in the mean for the
+// one-CTA kernel, by 8 % for the pairs; the variant it chooses takes 1.4 % longer than the best in the mean and 20 % at
+// most, and 0.7 and 17 % where sums may be 1024 deep. Measured at what the choice turns on: 128 x 2304 x 768 5.0 us in
+// tiles of 16, 6.2 on pairs; 128 x 19456 x 2560 17.8 in tiles of 128, 37.0 of 16, 20.0 on pairs; 12 x 2560 x 9728 10.1
+// split four ways, 19.4 whole; 1000 x 4096 x 2560 13.6 on pairs, 16.3 in tiles of 128; 768 x 1152 x 8191 17.6 on pairs
+// split four ways, 20.0 whole (in halves); 4097 x 16384 x 2048 100.5 on pairs, 106.2 as two sums.
 static float cost_1cta(int M, int N, int K, int tn, int splits) {
   // launch, set-up and epilogue; 1000 deep of one CTA on an SM; of one of two
   constexpr float kSet[4] = {3.6f, 4.1f, 6.2f, 8.2f}, kOne[4] = {1.67f, 1.77f, 1.85f, 2.36f},
@@ -525,12 +526,12 @@ static float cost_1cta(int M, int N, int K, int tn, int splits) {
 }
 // (The plan depends on the sizes alone, not on the device's count of pairs: storage is sized by it, and it fixes the
 // order of sums.)
-static float cost_2cta(int M, int N, int K, int splits, int deepest) {
+static float cost_2cta(int M, int N, int K, int splits, int deepest, bool halves) {
   constexpr float pairs = 74.f;
   const float tiles = 1.f * ((M + 255) / 256) * ((N + 255) / 256) * splits;
   const float each = 1e-3f * K / splits, full = floorf(tiles / pairs), rest = tiles - full * pairs;
-  // (a last wave of few tiles runs in halves)
-  const float waves = full + (rest == 0.f ? 0.f : (splits == 1 && 2.f * rest <= pairs ? 0.55f : 1.f));
+  // `halves`: a last wave of few tiles runs in those
+  const float waves = full + (rest == 0.f ? 0.f : (halves && splits == 1 && 2.f * rest <= pairs ? 0.55f : 1.f));
   // (the issuer waits for the end of a sum and the first of its columns before it starts the next: 0.6 to 0.8 us)
   const float joins = 0.6f * (block_2cta_sums(K, deepest) - 1);
   return 4.85f + waves * (1.83f + joins + 2.4f * each) +
@@ -552,17 +553,20 @@ BlockPlan block_plan(int M, int N, int K, bool aligned, int deepest) {
   if (!aligned) return best;
   for (int s = 1; s <= 8; ++s) {
     if (!block_2cta_splits_ok(K, s) || (s > 1 && deepest > 0 && block_2cta_depth(K, s) > deepest)) continue;
-    const float c = cost_2cta(M, N, K, s, s > 1 ? 0 : deepest);
+    const float c = cost_2cta(M, N, K, s, s > 1 ? 0 : deepest, true);
     if (c < best.cost) best = BlockPlan{1, 0, s, c, deepest};
   }
   return best;
 }
 
 // The fused projection and activation on CTA pairs, or the products and a launch that activates and casts
-// (measured at 24 x 9728 x 2560: 25.8 and 17.0 us; 500 x 4096 x 1024: 13.5 and 15.5).
+// (the gated kernel runs no halves). Measured, SwiGLU, one or the other: 64 x 9728 x 2560 22.6 / 14.8 + 3.6 us, 500 x 4096 x
+// 1024 10.3 / 10.1 + 5.7, 4097 x 8192 x 2048 100.6 / 100.5 + 41.7. The variant it chooses takes 0.4 % longer than the better
+// one in the mean and 9 % at most (67 sizes, rows 12 to 4097). tanh-GELU (11.5 / 10.1 + 7.7 at the second size) adds as
+// much to the one as to the other.
 bool block_glu_fused(int T, int I, int K, int deepest) {
-  const float fused = cost_2cta(T, 2 * I, K, 1, deepest) + 1.f;
-  return fused < block_plan(T, 2 * I, K, true, deepest).cost + 2.5f + 2e-6f * T * float(I);
+  return cost_2cta(T, 2 * I, K, 1, deepest, false) <
+         block_plan(T, 2 * I, K, true, deepest).cost + 3.5f + 1.16e-6f * T * float(I);
 }
 
 size_t block_plan_bytes(const BlockPlan& p, int M, int N) {
