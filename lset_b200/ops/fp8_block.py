@@ -39,10 +39,10 @@ class Fp8BlockTensor:
     b % 4]`` is the exponent (1 to 254, biased by 127) of the scale of columns ``128 b .. 128 b + 127`` of row ``r``;
     bytes of blocks that a row does not have are not read.
 
-    The two are checked here, once; a product takes them as they are, and looks again only where one has another layout
-    than it had (its ``.data`` exchanged). Copies (``copy``, ``pickle``) are made and checked anew, on memory of their own.
+    The two are checked here, once; a product takes them as they are, and looks again where one lies elsewhere than it
+    did (its ``.data`` exchanged). Copies (``copy``, ``pickle``) are made and checked anew, on memory of their own.
     """
-    __slots__ = ("_data", "_cols", "_scales", "_e5m2", "_ld", "_group", "_layout")
+    __slots__ = ("_data", "_cols", "_scales", "_e5m2", "_seen", "_at")
 
     def __init__(self, data: torch.Tensor, cols: int, scales: torch.Tensor, e5m2: bool = False):
         self._data, self._cols, self._scales, self._e5m2 = data, cols, scales, bool(e5m2)
@@ -52,8 +52,9 @@ class Fp8BlockTensor:
         data, cols, scales = self._data, self._cols, self._scales
         if data.dtype is not torch.uint8 or scales.dtype is not torch.uint8 or data.dim() != 2 or scales.dim() != 3:
             raise TypeError("data is a 2-D and scales a 3-D tensor of bytes")
-        layout = data.shape, data.stride(), scales.shape, scales.stride()
-        (rows, width), (ld, step), (groups, s_rows, four), (s_group, s_row, s_byte) = layout
+        strides, s_strides = data.stride(), scales.stride()
+        (rows, width), (ld, step) = data.shape, strides
+        (groups, s_rows, four), (s_group, s_row, s_byte) = scales.shape, s_strides
         if not 0 <= cols <= width or groups != (cols + 511) // 512 or s_rows != rows or four != 4:
             raise ValueError(f"data {tuple(data.shape)} with {cols} columns and scales {tuple(scales.shape)} do not "
                              f"belong together")
@@ -65,25 +66,26 @@ class Fp8BlockTensor:
             raise ValueError("the bytes of a row lie next to one another")
         if rows and groups and (s_byte != 1 or s_row != 4 or s_group % 4 or s_group < 4 * rows):
             raise ValueError("the scales of four blocks lie next to one another, row by row")
-        if data.is_cuda and (ld % 16 or data.data_ptr() % 16 or scales.data_ptr() % 4) and width and rows:
+        ptr, s_ptr = data.data_ptr(), scales.data_ptr()
+        if data.is_cuda and (ld % 16 or ptr % 16 or s_ptr % 4) and width and rows:
             raise ValueError("rows start at multiples of 16 bytes, their scales at multiples of 4")
         if data.get_device() != scales.get_device():
             raise ValueError("data and scales are on one device")
-        self._ld, self._group, self._layout = ld, s_group // 4, layout
+        if not (ptr and s_ptr) and data.numel() and scales.numel():
+            raise ValueError("the memory of a block-scaled matrix was released")
+        self._seen = ptr, s_ptr, strides, s_strides
+        # as the launchers take it: bytes, their row stride, scale words, words of a group of four blocks
+        self._at = ptr, ld, s_ptr, s_group // 4
 
     def __reduce__(self):
         return Fp8BlockTensor, (self._data, self._cols, self._scales, self._e5m2)
 
     @property
     def _where(self):
-        """As the launchers take it: bytes, their row stride, scale words, words of a group of four blocks."""
         data, scales = self._data, self._scales
-        ptr, s_ptr = data.data_ptr(), scales.data_ptr()
-        if ptr & 15 or s_ptr & 3 or (data.shape, data.stride(), scales.shape, scales.stride()) != self._layout:
+        if (data.data_ptr(), scales.data_ptr(), data.stride(), scales.stride()) != self._seen:
             self._check()
-        if not (ptr and s_ptr) and data.numel() and scales.numel():
-            raise ValueError("the memory of a block-scaled matrix was released")
-        return ptr, self._ld, s_ptr, self._group
+        return self._at
 
     data = property(lambda self: self._data)
     cols = property(lambda self: self._cols)
