@@ -301,6 +301,25 @@ __global__ void __launch_bounds__(256, 4)
   if (WANT) cast_tile<TILED, E5M2, WANT, 2>(v, sm, r0, c0, R, C, out, out_t);
 }
 
+// Column sums of each 128 rows of x (fp32, rows ldx elements apart), always added in the same order: the gradient of a
+// bias behind fp32 activations, whose dy is rounded for the products alone. Bound by memory.
+__global__ void __launch_bounds__(2 * kTile)
+    block_colsum_kernel(const float* __restrict__ x, int R, int C, long long ldx, float* __restrict__ colsum) {
+  __shared__ float part[kTile];
+  pdl_wait();
+  pdl_trigger();
+  const int tiles_c = (C + kTile - 1) / kTile, rt = blockIdx.x / tiles_c;
+  const int r0 = rt * kTile, c = (blockIdx.x - rt * tiles_c) * kTile + threadIdx.x % kTile, odd = threadIdx.x / kTile;
+  float t = 0.f;
+  if (c < C) {
+#pragma unroll 8
+    for (int r = r0 + odd; r < min(r0 + kTile, R); r += 2) t += x[r * ldx + c];
+  }
+  if (odd) part[threadIdx.x % kTile] = t;
+  __syncthreads();
+  if (!odd && c < C) colsum[(long long)rt * C + c] = t + part[threadIdx.x];
+}
+
 // Several casts in one launch, both layouts of each: the activations and the weights of a layer, which do not wait for one
 // another. Measured for x [257, 1024] and w [2048, 1024]: 3.9 + 3.3 us in launches of their own, with 1.6 between them;
 // x [4097, 2048] with w [16384, 2048] and [2048, 8192]: 11.0 + 26.9 + 20.0 us, 38 together.
@@ -498,6 +517,13 @@ int block_cast(const void* x, int R, int C, long long ldx, int tiled, int e5m2, 
   return launch_pdl(kern, dim3(grid), dim3(256), 0, stream, pdl_enabled(4LL * R * C), 1,
                     static_cast<const bf16*>(x), R, C, ldx, block_out(out), block_out(out_t, kb0_t), colsum,
                     (C + kTile - 1) / kTile);
+}
+
+int block_colsum(const float* x, int R, int C, long long ldx, float* colsum, cudaStream_t stream) {
+  const unsigned grid = cast_grid(R, C);
+  if (R <= 0 || C <= 0 || grid == 0) return -3;
+  return launch_pdl(block_colsum_kernel, dim3(grid), dim3(2 * kTile), 0, stream, pdl_enabled(4LL * R * C), 1, x, R, C, ldx,
+                    colsum);
 }
 
 int block_casts(const BlockCast* jobs, int n, cudaStream_t stream) {

@@ -69,6 +69,8 @@ int block_gemm_glu(int kind, int deepest, const BlockMat& A, const BlockMat& Wg,
 // [ceil(R / 128)][C], the column sums of each 128 rows of x (null: not wanted).
 int block_cast(const void* x, int R, int C, long long ldx, int tiled, int e5m2, const BlockMat& out,
                const BlockMat& out_t, int kb0_t, float* colsum, cudaStream_t stream);
+// The same column sums of an fp32 matrix by themselves.
+int block_colsum(const float* x, int R, int C, long long ldx, float* colsum, cudaStream_t stream);
 // Up to kMaxCasts casts to e4m3 in one launch (where both layouts of all are wanted).
 enum { kMaxCasts = 4 };
 struct BlockCast {

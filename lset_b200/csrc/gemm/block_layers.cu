@@ -219,14 +219,17 @@ extern "C" int lb_linear_kept_fwd(const void* x, long long ldx, const void* w, l
 }
 
 // dx [T, K] = dy · w, dw [N, K] = or += dyᵀ · x, db [N] = column sums of dy (rows lddy elements apart), of those
-// that `need` names, from what the forward saved. dx_mode, db_mode: 0 or 1.
-extern "C" int lb_linear_block_bwd(const void* dy, long long lddy, int T, int K, int N, int need, void* saved,
+// that `need` names, from what the forward saved. dx_mode, db_mode: 0 or 1. dy32 (rows lddy32 elements apart; null:
+// none): dy before it was rounded to bf16, which db then is the sum of.
+extern "C" int lb_linear_block_bwd(const void* dy, long long lddy, const float* dy32, long long lddy32, int T, int K, int N, int need, void* saved,
                                    void* tmp, void* dx, int dx_mode, void* dw, int dw_mode, void* db, int db_mode,
                                    int* status, void* stream_) {
   if (T <= 0 || K <= 0 || N <= 0) return -3;
   const LinearStorage s = linear_storage(T, K, N, need, saved, tmp);
   Call c{status, reinterpret_cast<cudaStream_t>(stream_), s.ws_bwd};
-  c.run([&] { return block_cast(dy, T, N, lddy, 0, 0, s.dy, s.dy_t, 0, s.colsum, c.stream); });
+  const bool apart = dy32 != nullptr && (need & 4);
+  c.run([&] { return block_cast(dy, T, N, lddy, 0, 0, s.dy, s.dy_t, 0, apart ? nullptr : s.colsum, c.stream); });
+  if (apart) c.run([&] { return block_colsum(dy32, T, N, lddy32, s.colsum, c.stream); });
   if (need & 1) c.product(s.dy, s.w_t, Out{dx, dx_mode}, T, K, N, K);
   if (need & 2) c.product(s.dy_t, s.x_t, Out{dw, dw_mode}, N, K, T, K);
   if (need & 4)

@@ -112,7 +112,7 @@ _SIGNATURES = {
     "lb_gemm_block": [_P, _P, _P, _I, _I, _I, _L, _L, _L, _I, _I, _P, _L, _P, _L, _I, _I, _P, _P, _L, _P, _P],
     "lb_linear_block_bytes": [_I] * 4 + [_P],
     "lb_linear_block_fwd": [_P, _L, _P, _L, _P, _I, _I, _I, _I, _I] + [_P] * 5,
-    "lb_linear_block_bwd": [_P, _L, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _P, _I, _P, _P],
+    "lb_linear_block_bwd": [_P, _L, _P, _L, _I, _I, _I, _I, _P, _P, _P, _I, _P, _I, _P, _I, _P, _P],
     "lb_linear_kept_bytes": [_I] * 3,
     "lb_linear_kept_fwd": [_P, _L, _P, _L, _P, _L, _I, _P, _I, _I, _I, _I, _P, _P, _P, _P],
     "lb_mlp_block_bytes": [_I] * 4 + [_P],
@@ -444,6 +444,7 @@ class _LinearFp8Block(torch.autograd.Function):
             return dx, dw, db
         saved, dev = kept[0], dy.device
         with _on_device(dy, w):
+            dy32 = dy2.contiguous() if need & 4 and dy2.dtype is torch.float32 else None
             dy2 = _aligned(dy2)
             x_mode = x_dtype is torch.float32
             if need & 1:
@@ -453,9 +454,9 @@ class _LinearFp8Block(torch.autograd.Function):
             if need & 4:
                 db = torch.empty(N, dtype=torch.float32 if b_mode else torch.bfloat16, device=dev)
             tmp = _bytes(_linear_bytes(T, K, N, need)[2], dev)
-            _call("lb_linear_block_bwd", dy2.data_ptr(), dy2.stride(0), T, K, N, need, saved.data_ptr(), tmp.data_ptr(),
-                  nv.ptr(dx), x_mode, nv.ptr(g), g_mode, nv.ptr(db), b_mode, _status_ptr(dev), nv.stream_ptr())
-            nv.count_launch(1 + bool(need & 1) + bool(need & 2) + bool(need & 4))
+            _call("lb_linear_block_bwd", dy2.data_ptr(), dy2.stride(0), nv.ptr(dy32), N, T, K, N, need, saved.data_ptr(),
+                  tmp.data_ptr(), nv.ptr(dx), x_mode, nv.ptr(g), g_mode, nv.ptr(db), b_mode, _status_ptr(dev), nv.stream_ptr())
+            nv.count_launch(1 + bool(need & 1) + bool(need & 2) + bool(need & 4) + (dy32 is not None))
             if need & 2:
                 dw = _returned(w, g, g_mode)
             if need & 1 and dx.dtype is not x_dtype:
@@ -470,8 +471,9 @@ def linear_fp8_block(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) ->
 
     ``w [N, K]`` is a bf16 (or fp32) weight, cast here for the three products of a training step, or an
     ``Fp8BlockTensor`` from ``quantize_fp8_block(w, tile=True)`` that an inference program keeps (no gradients
-    then). ``x`` is ``[..., K]``; ``y`` has its type if that is bf16 or fp32, else bf16. On the GPU ``K`` and
-    ``N`` are multiples of 8. The weight gradient goes into the fp32 accumulator of the sharding runtime
+    then). ``x`` is ``[..., K]``; ``y`` has its type if that is bf16 or fp32, else bf16. Operands (``x``, ``w``, the gradient
+    of ``y``) of other types are rounded to bf16 on their way to 8 bits, and so is ``bias``; its gradient is the sum of
+    the gradient of ``y`` as it comes. On the GPU ``K`` and ``N`` are multiples of 8. The weight gradient goes into the fp32 accumulator of the sharding runtime
     where the weight has one.
     """
     N, K = w.shape

@@ -642,3 +642,60 @@ def test_the_gated_kernel_is_chosen_where_it_is_the_faster():
     product and an activation (whose products then have storage), 500 of 4096 on 1024 10.3 for 15.8."""
     assert fb._mlp_kept_bytes(64, 2560, 9728) >= 4 * 64 * 9728
     assert fb._mlp_kept_bytes(500, 1024, 4096) < 4 * 500 * 4096
+
+
+def _sums(a, b, depth):
+    """What fp32 sums of |a| |b|ᵀ that deep may be off (_check_product says why)."""
+    return (depth // 32 + 3) * 2.0 ** -22 * (a.abs() @ b.abs().t())
+
+
+@pytest.mark.parametrize("T", [1, 5, 129, 700])
+@pytest.mark.parametrize("bias_type", [torch.float32, torch.bfloat16])
+def test_values_of_an_fp32_linear_layer(T, bias_type):
+    """fp32 activations and weights: operands are rounded to bf16 on their way to 8 bits, results are fp32, and the
+    gradient of the bias is the sum of dy as it comes."""
+    K, N = 272, 136
+    g = torch.Generator("cuda").manual_seed(T)
+    x, w, dy = (torch.randn(*s, generator=g, device="cuda") for s in ((T, K), (N, K), (T, N)))
+    b = torch.randn(N, generator=g, device="cuda").to(bias_type)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = fb.linear_fp8_block(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    nv.check_status()
+    xr, xc, dr, dc, wv = _value(x, 1, 128), _value(x, 128, 1), _value(dy, 1, 128), _value(dy, 128, 1), _value(w, 128, 128)
+    bv = b.detach().to(torch.bfloat16).double()
+    for got, want, off in ((y.detach(), xr @ wv.t() + bv, _sums(xr, wv, K)), (dx, dr @ wv, _sums(dr, wv.t(), N)),
+                           (dw, dc.t() @ xc, _sums(dc.t(), xc.t(), T))):
+        assert got.dtype == torch.float32
+        assert ((got.double() - want).abs() <= 2.0 ** -23 * want.abs() + off).all()
+    want = dy.double().sum(0)
+    assert db.dtype == bias_type
+    half = 2.0 ** -8 if bias_type is torch.bfloat16 else 2.0 ** -23
+    assert ((db.double() - want).abs() <= half * want.abs() + (130 + T // 128) * 2.0 ** -24 * dy.double().abs().sum(0)).all()
+    (only,) = torch.autograd.grad(fb.linear_fp8_block(x, w, b), b, dy.expand(T, N))
+    assert torch.equal(only, db)
+    (ones,) = torch.autograd.grad(fb.linear_fp8_block(x, w, b).sum(), b)
+    assert (ones == T).all()
+
+
+@pytest.mark.parametrize("T", [1, 130])
+def test_values_of_an_fp32_gated_block(T):
+    """fp32 activations, weights and accumulators: what bf16 ones of the same values give, rounded to bf16 in between."""
+    H, I = 264, 256
+    x, dy = _rand(T, H, spread=0.5), _rand(T, H, seed=1, spread=1.0)
+    w, wd = _rand(2 * I, H, seed=2, spread=0.3) * H ** -0.5, _rand(H, I, seed=3, spread=0.3) * I ** -0.5
+    leaves = [t.requires_grad_() for t in (x, w, wd)]
+    y = fb.gated_mlp_fp8_block(x, w, None, wd)
+    want = torch.autograd.grad(y, leaves, dy)
+    fp32 = [t.detach().float().requires_grad_() for t in leaves]
+    z = fb.gated_mlp_fp8_block(fp32[0], fp32[1], None, fp32[2])
+    got = torch.autograd.grad(z, fp32, dy.float())
+    assert z.dtype == torch.float32 and torch.equal(z, y.float()) and torch.equal(got[0], want[0].float())
+    for a, b in zip(got[1:], want[1:]):      # fp32 sums, and those rounded to bf16
+        assert a.dtype == torch.float32 and torch.equal(a.to(torch.bfloat16), b)
+    for t in leaves[1:]:
+        t.main_grad = torch.full(t.shape, 2.0, device="cuda")
+    fb.gated_mlp_fp8_block(x, w, None, wd).backward(dy)
+    for t, a in zip(leaves[1:], got[1:]):    # added to what is there: half a step of the sum's type
+        assert t.grad is None and ((t.main_grad - 2 - a).abs() <= 2.0 ** -23 * (2 + a.abs())).all()
+    nv.check_status()
