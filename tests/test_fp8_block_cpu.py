@@ -471,3 +471,16 @@ def test_exchanged_memory_is_looked_at_again():
     q.data.untyped_storage().resize_(0)
     with pytest.raises(ValueError, match="released"):
         q._where
+
+
+def test_products_of_more_rows_than_are_counted_are_refused(monkeypatch):
+    """The kernels' sizes are ints of 32 bits, which 2^31 rows would pass (0 columns: nothing is stored here)."""
+    many = fb.Fp8BlockTensor(torch.empty(1 << 31, 0, dtype=torch.uint8), 0, torch.empty(0, 1 << 31, 4, dtype=torch.uint8))
+    few = fb.Fp8BlockTensor(torch.empty(2, 0, dtype=torch.uint8), 0, torch.empty(0, 2, 4, dtype=torch.uint8))
+    monkeypatch.setattr(fb.nv, "use_native", lambda *t: True)
+    made = []
+    monkeypatch.setattr(fb, "_on_device", lambda *t: made.append(t))
+    for a, b in ((many, few), (few, many)):
+        with pytest.raises(ValueError, match="more rows or columns"):
+            fb.matmul_fp8_block(a, b)
+    assert not made
