@@ -483,7 +483,8 @@ def linear_fp8_block(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) ->
         raise ValueError(f"bias has to be [{N}]")
     if not isinstance(w, Fp8BlockTensor):
         if x.numel() == 0 or N == 0:
-            return torch.nn.functional.linear(x, w.to(x.dtype), None if bias is None else bias.to(x.dtype))
+            y = torch.nn.functional.linear(x, w.to(x.dtype), None if bias is None else bias.to(x.dtype))
+            return y if x.dtype is torch.float32 else y.to(torch.bfloat16)
         if not torch.is_grad_enabled():      # nothing is kept for a backward then
             x, w, bias = x.detach(), w.detach(), None if bias is None else bias.detach()
         return _LinearFp8Block.apply(x, w, bias)
@@ -653,7 +654,8 @@ def gated_mlp_fp8_block(x: torch.Tensor, w_gate, w_up, w_down, kind: str = "swig
     if not any(kept):
         if x.numel() == 0:
             zero = sum(w.sum() for w in (w_gate, w_up, w_down) if w is not None) * 0
-            return x * zero.to(x.dtype)      # keeps the graph: gradients of zero
+            y = x * zero.to(x.dtype)      # keeps the graph: gradients of zero
+            return y if x.dtype is torch.float32 else y.to(torch.bfloat16)
         if not torch.is_grad_enabled():      # nothing is kept for a backward then
             x, w_gate, w_up, w_down = (t if t is None else t.detach() for t in (x, w_gate, w_up, w_down))
         return _GatedMlpFp8Block.apply(x, w_gate, w_up, w_down, kind)

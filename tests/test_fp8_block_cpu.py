@@ -484,3 +484,16 @@ def test_products_of_more_rows_than_are_counted_are_refused(monkeypatch):
         with pytest.raises(ValueError, match="more rows or columns"):
             fb.matmul_fp8_block(a, b)
     assert not made
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32, torch.bfloat16, torch.float64])
+def test_results_of_empty_batches_have_the_type_of_others(dtype):
+    w, wd = torch.randn(256, 64, requires_grad=True), torch.randn(64, 128, requires_grad=True)
+    b = torch.randn(256)
+    for fn in (lambda x: fb.linear_fp8_block(x, w, b), lambda x: fb.gated_mlp_fp8_block(x, w, None, wd)):
+        empty, some = torch.empty(0, 64, dtype=dtype, requires_grad=True), torch.randn(3, 64).to(dtype)
+        y, z = fn(empty), fn(some)
+        assert y.dtype == z.dtype == (torch.float32 if dtype is torch.float32 else torch.bfloat16)
+        assert y.shape == (0, z.shape[1])
+        y.sum().backward()
+        assert empty.grad.shape == (0, 64) and empty.grad.dtype == dtype and not w.grad.any()
