@@ -308,6 +308,8 @@ def matmul_fp8_block(a: Fp8BlockTensor, b: Fp8BlockTensor, *, out: Optional[torc
         if out is None:
             return c.to(out_dtype)
         return out.add_(c) if accumulate else out.copy_(c)
+    if max(M, N, K) >= _MOST:
+        raise ValueError(f"more rows or columns than the kernels count: {M}, {N}, {K}")
     with _on_device(a.data, b.data, out, bias):
         if out is None:
             out = torch.empty(M, N, dtype=out_dtype, device=a.data.device)
