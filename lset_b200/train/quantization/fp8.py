@@ -165,6 +165,15 @@ class Fp8KeptLinear(nn.Module):
     def forward(self, x):
         return fb.linear_fp8_block(x, self.fp8_block_weight(), self.bias)
 
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs):
+        for name in ("weight", "scales"):      # a copy into bytes would cut the values of a weight off
+            t = state_dict.get(prefix + name)
+            if t is not None and t.dtype is not torch.uint8:
+                error_msgs.append(f"{prefix}{name} holds 8-bit values and is given {t.dtype} ones: load a model's weights "
+                                  f"before apply_fp8_inference")
+                return
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
+
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
 

@@ -497,3 +497,16 @@ def test_results_of_empty_batches_have_the_type_of_others(dtype):
         assert y.shape == (0, z.shape[1])
         y.sum().backward()
         assert empty.grad.shape == (0, 64) and empty.grad.dtype == dtype and not w.grad.any()
+
+
+def test_weights_of_another_type_are_not_loaded_into_bytes():
+    from lset_b200.train.quantization.fp8 import apply_fp8_inference
+
+    plain = _tiny().state_dict()
+    model = apply_fp8_inference(_tiny())
+    before = {k: v.clone() for k, v in model.state_dict().items()}
+    for strict in (True, False):      # not strict, missing scales alone would pass
+        with pytest.raises(RuntimeError, match="before apply_fp8_inference"):
+            model.load_state_dict(plain, strict=strict)
+    assert all(torch.equal(v, before[k]) for k, v in model.state_dict().items() if v.dtype is torch.uint8)
+    model.load_state_dict(before)
