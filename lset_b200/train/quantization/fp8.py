@@ -162,6 +162,9 @@ class Fp8KeptLinear(nn.Module):
     def fp8_block_weight(self):
         return fb.Fp8BlockTensor(self.weight, self.in_features, self.scales)
 
+    def dequantized_weight(self) -> torch.Tensor:
+        return self.fp8_block_weight().dequantize()
+
     def forward(self, x):
         return fb.linear_fp8_block(x, self.fp8_block_weight(), self.bias)
 
@@ -180,8 +183,10 @@ class Fp8KeptLinear(nn.Module):
 
 def apply_fp8_inference(model: nn.Module) -> nn.Module:
     """Replaces, in place, every eligible linear layer of a model that only encodes by an ``Fp8KeptLinear``. Separate
-    gate and up projections of a gated MLP become one fused layer, which the fused operator takes."""
+    gate and up projections of a gated MLP become one fused layer, which the fused operator takes. Of a layer with
+    a LoRA adapter the base is replaced; the adapter stays as it is."""
     from ...models.layers import GatedMLP
+    from ..lora import LoRALinear
 
     for mod in list(model.modules()):
         if (isinstance(mod, GatedMLP) and not mod.fused_gate_up
@@ -192,6 +197,8 @@ def apply_fp8_inference(model: nn.Module) -> nn.Module:
             del mod.gate_proj, mod.up_proj
     for mod in list(model.modules()):
         for name, child in list(mod.named_children()):
+            if isinstance(mod, LoRALinear) and name != "base_linear":
+                continue
             if isinstance(child, nn.Linear) and type(child).__name__ == "Linear" and _eligible(child):
                 setattr(mod, name, Fp8KeptLinear(child.weight, child.bias))
     return model

@@ -510,3 +510,25 @@ def test_weights_of_another_type_are_not_loaded_into_bytes():
             model.load_state_dict(plain, strict=strict)
     assert all(torch.equal(v, before[k]) for k, v in model.state_dict().items() if v.dtype is torch.uint8)
     model.load_state_dict(before)
+
+
+def test_adapters_stay_as_they_are_and_merge_with_the_values_of_kept_weights():
+    from lset_b200.train.lora import LoRALinear, apply_lora
+    from lset_b200.train.quantization.fp8 import Fp8KeptLinear, apply_fp8_inference
+
+    model, ids = _tiny(), torch.randint(0, 97, (2, 9), generator=torch.Generator().manual_seed(0))
+    apply_lora(model, r=16, target_modules=["q_proj", "down_proj"])
+    for m in model.modules():
+        if isinstance(m, LoRALinear):
+            torch.nn.init.normal_(m.lora_B.weight, std=0.05)
+    with torch.no_grad():
+        want = model(ids)["hidden_states"]
+        merged = [m.merged_weight() for m in model.modules() if isinstance(m, LoRALinear)]
+        apply_fp8_inference(model)
+        got = model(ids)["hidden_states"]
+        layers = [m for m in model.modules() if isinstance(m, LoRALinear)]
+        assert len(layers) == len(merged) == 4
+        for m, w in zip(layers, merged):
+            assert isinstance(m.base_linear, Fp8KeptLinear) and type(m.lora_A).__name__ == "Linear"
+            assert float((m.merged_weight() - w).norm() / w.norm()) < 2.0 ** -4      # half a step of e4m3 at most
+    assert float(torch.nn.functional.cosine_similarity(got, want, dim=-1).min()) > 0.98
