@@ -699,3 +699,129 @@ def test_values_of_an_fp32_gated_block(T):
     for t, a in zip(leaves[1:], got[1:]):    # added to what is there: half a step of the sum's type
         assert t.grad is None and ((t.main_grad - 2 - a).abs() <= 2.0 ** -23 * (2 + a.abs())).all()
     nv.check_status()
+
+
+@pytest.mark.parametrize("M,N,K", SPLIT)
+def test_split_products_into_given_outputs(M, N, K):
+    a, _ = fb.quantize_fp8_block(_rand(M, K, spread=1.0))
+    b, _ = fb.quantize_fp8_block(_rand(N, K, seed=1, spread=1.0), tile=True)
+    for dt in (torch.bfloat16, torch.float32):
+        wide = torch.full((M + 2, N + 24), 7.0, dtype=dt, device="cuda")
+        out = wide[1:M + 1, 8:N + 8]
+        assert fb._product_bytes(M, N, K, N + 24) >= 2 * 4 * M * N
+        fb.matmul_fp8_block(a, b, out=out)
+        _check_product(out, a, b)
+        out.fill_(7)
+        assert (wide == 7).all()                 # nothing around it
+    base = torch.randn(M, N, device="cuda") * K ** 0.5
+    out = base.clone()
+    fb.matmul_fp8_block(a, b, out=out, accumulate=True)
+    _check_product(out, a, b, base=base)
+    nv.check_status()
+
+
+def test_split_weight_gradients_of_a_long_batch():
+    T, K, N = 16384, 768, 768
+    assert fb._product_bytes(N, K, T, K) >= 2 * 4 * N * K
+    x, w, dy = _rand(T, K, spread=0.5), _rand(N, K, seed=1, spread=0.5), _rand(T, N, seed=2, spread=0.5)
+    a, b = _value(dy, 128, 1).t(), _value(x, 128, 1).t()
+    want, off = a @ b.t(), _sums(a, b, T)
+    x.requires_grad_(), w.requires_grad_()
+    y = fb.linear_fp8_block(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy, retain_graph=True)
+    assert ((dw.double() - want).abs() <= 2.0 ** -8 * want.abs() + off).all()
+    wv, dr = _value(w, 128, 128), _value(dy, 1, 128)
+    assert ((dx.double() - dr @ wv).abs() <= 2.0 ** -8 * (dr @ wv).abs() + _sums(dr, wv.t(), N)).all()
+    w.main_grad = torch.full((N, K), 3.0, device="cuda")
+    for n in (1, 2):
+        y.backward(dy, retain_graph=True)
+        assert w.grad is None
+        assert ((w.main_grad.double() - 3 - n * want).abs() <= n * (2.0 ** -23 * (3 + n * want.abs()) + off)).all()
+    nv.check_status()
+
+
+@pytest.mark.parametrize("T", [1, 17, 129, 1000, 2600])
+@pytest.mark.parametrize("K,N,bias", [(136, 264, True), (640, 72, True), (2568, 1032, False)])
+def test_linear_layers_value_by_value(T, K, N, bias):
+    x, w, dy = _rand(T, K, spread=1.0), _rand(N, K, seed=1, spread=0.5), _rand(T, N, seed=2, spread=1.0)
+    b = _rand(N, seed=3, spread=0.5) if bias else None
+    leaves = [t.requires_grad_() for t in (x, w, b) if t is not None]
+    y = fb.linear_fp8_block(x, w, b)
+    got = [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+    nv.check_status()
+    xr, xc, dr, dc, wv = _value(x, 1, 128), _value(x, 128, 1), _value(dy, 1, 128), _value(dy, 128, 1), _value(w, 128, 128)
+    want = [(xr @ wv.t() + (0 if b is None else b.detach().double()), _sums(xr, wv, K)), (dr @ wv, _sums(dr, wv.t(), N)),
+            (dc.t() @ xc, _sums(dc.t(), xc.t(), T))]
+    if bias:
+        want.append((dy.double().sum(0), (130 + T // 128) * 2.0 ** -24 * dy.double().abs().sum(0)))
+    for a, (c, off) in zip(got, want):
+        assert ((a.double() - c).abs() <= 2.0 ** -8 * c.abs() + off).all()
+
+
+def _rows_close(got, a, b, flips=2):
+    """Each row of ``got`` beside ``a @ b``: half a step of bf16, what its sums may be off, and ``flips`` values of a's row that
+    fell to the other side of a rounding to 8 bits, by 2^-3 of themselves."""
+    want = a @ b
+    off = ((a.shape[1] // 32 + 3) * 2.0 ** -22) * (a.abs() @ b.abs())
+    one = (a.abs() * b.norm(dim=1)).amax(dim=1)
+    bound = 2.0 ** -8 * want.norm(dim=1) + off.norm(dim=1) + flips * 2.0 ** -3 * one
+    err = (got.double() - want).norm(dim=1)
+    assert (err <= bound).all(), (int((err > bound).sum()), float((err / bound).max()))
+
+
+@pytest.mark.parametrize("kind", ["swiglu", "geglu"])
+@pytest.mark.parametrize("T,H,I", [(1, 264, 384), (33, 1032, 256), (129, 2568, 128), (333, 1152, 1280), (1500, 4104, 640),
+                                   (2600, 2048, 1024), (4097, 1288, 2432)])
+def test_gated_blocks_row_by_row(T, H, I, kind):
+    """Sums of one part and of several, few rows and many, ragged widths; gate and up products value by value, the rest by rows
+    (of weight gradients, by features)."""
+    x, dy = _rand(T, H, spread=0.5), _rand(T, H, seed=1, spread=0.5)
+    w, wd = _rand(2 * I, H, seed=2, spread=0.3) * H ** -0.5, _rand(H, I, seed=3, spread=0.3) * I ** -0.5
+    leaves = [t.requires_grad_() for t in (x, w, wd)]
+    y = fb.gated_mlp_fp8_block(x, w, None, wd, kind)
+    gu = y.grad_fn.saved_tensors[-1][:4 * T * I].view(torch.bfloat16).view(T, 2 * I).clone()
+    dx, dw, dwd = torch.autograd.grad(y, leaves, dy)
+    nv.check_status()
+    xr, xc, wv, dv = _value(x, 1, 128), _value(x, 128, 1), _value(w, 128, 128), _value(wd, 128, 128)
+    dr, dc = _value(dy, 1, 128), _value(dy, 128, 1)
+    want = xr @ wv.t()
+    assert ((gu.double() - want).abs() <= 2.0 ** -8 * want.abs() + _sums(xr, wv, H)).all()
+    leaf = gu.float().requires_grad_()
+    g, u = leaf[:, :I], leaf[:, I:]
+    act = torch.nn.functional.silu(g) if kind == "swiglu" else 0.5 * g * (
+        1 + torch.tanh(0.7978845608028654 * (g + 0.044715 * g * g * g)))
+    h = act * u
+    dh = (dr @ dv).to(torch.bfloat16).float()
+    (dgu,) = torch.autograd.grad(h, leaf, dh)
+    hb, db = h.detach().to(torch.bfloat16), dgu.to(torch.bfloat16)
+    _rows_close(y.detach(), _value(hb, 1, 128), dv.t())
+    _rows_close(dx, _value(db, 1, 128), wv)
+    _rows_close(dw, _value(db, 128, 1).t(), xc)
+    _rows_close(dwd.t(), _value(hb, 128, 1).t(), dc)
+    with torch.no_grad():
+        kept = [fb.quantize_fp8_block(t, tile=True)[0] for t in (w, wd)]
+        z = fb.gated_mlp_fp8_block(x, kept[0], None, kept[1], kind)
+    if H <= 1024:
+        assert torch.equal(z, y)       # (deeper, a step's gate and up are sums of parts)
+    _rows_close(z, _value(hb, 1, 128), dv.t(), flips=4)
+
+
+def test_a_deep_training_step_captured_and_replayed_on_another_stream():
+    T, H, I = 1300, 2056, 256
+    x, dy = _rand(T, H, spread=0.5), _rand(T, H, seed=1, spread=0.5)
+    w, wd = _rand(2 * I, H, seed=2, spread=0.3) * H ** -0.5, _rand(H, I, seed=3, spread=0.3) * I ** -0.5
+    x.requires_grad_(), w.requires_grad_(), wd.requires_grad_()
+    step = lambda: torch.autograd.grad(fb.gated_mlp_fp8_block(x, w, None, wd), (x, w, wd), dy)  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        want = [t.clone() for t in step()]
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for _ in range(3):
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    nv.check_status()
