@@ -532,3 +532,63 @@ def test_adapters_stay_as_they_are_and_merge_with_the_values_of_kept_weights():
             assert isinstance(m.base_linear, Fp8KeptLinear) and type(m.lora_A).__name__ == "Linear"
             assert float((m.merged_weight() - w).norm() / w.norm()) < 2.0 ** -4      # half a step of e4m3 at most
     assert float(torch.nn.functional.cosine_similarity(got, want, dim=-1).min()) > 0.98
+
+
+def _tp_model():
+    from lset_b200.models import Qwen3Config, Qwen3Decoder
+    from lset_b200.models.layers import init_normal_
+    from lset_b200.train.quantization.fp8 import apply_fp8_training
+
+    torch.manual_seed(15)
+    cfg = Qwen3Config(vocab_size=97, hidden_size=64, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim=16)
+    model = Qwen3Decoder(cfg, fused_projections=False)
+    init_normal_(model, 0.05)
+    return apply_fp8_training(model, "block128"), cfg, torch.randint(0, 97, (2, 9))
+
+
+def _tp_worker(rank, world, port, out_dir):
+    import os
+
+    import torch.distributed as dist
+
+    from lset_b200.dist.tp import apply_tp
+    from lset_b200.models.parallel_plan import decoder_tp_plan
+
+    os.environ.update(RANK=str(rank), WORLD_SIZE=str(world), MASTER_ADDR="127.0.0.1", MASTER_PORT=str(port))
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    model, cfg, ids = _tp_model()
+    apply_tp(model, dist.group.WORLD, decoder_tp_plan(cfg))
+    seen = []
+    real = fb.gated_mlp_fp8_block
+    fb.gated_mlp_fp8_block = lambda *a: seen.append(a) or real(*a)
+    out = model(ids)["hidden_states"]
+    out.pow(2).sum().backward()
+    if rank == 0:
+        torch.save({"out": out.detach(), "grad": model.layers[0].mlp.down_proj.weight.grad, "calls": len(seen)},
+                   os.path.join(out_dir, "tp.pt"))
+    dist.barrier()
+    dist.destroy_process_group()
+
+
+def test_tensor_parallel_layers_run_one_by_one(tmp_path):
+    """Shards of 256 features, which the gated operator would take: its partial sums would miss the all-reduce behind the
+    down projection and the one in front of the gate's backward, so the layers' own forwards run. Blocks of 128 lie within
+    a shard, and partial sums are what the shards add to in either case, but for where they are rounded."""
+    import socket
+
+    import torch.multiprocessing as mp
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    mp.spawn(_tp_worker, args=(2, port, str(tmp_path)), nprocs=2, join=True)
+    got = torch.load(tmp_path / "tp.pt", weights_only=False)
+    model, _, ids = _tp_model()
+    out = model(ids)["hidden_states"]
+    out.pow(2).sum().backward()
+    assert got["calls"] == 0
+    # o_proj's blocks of 128 inputs become one of 32 a rank, with scales of their own: an 8-bit step, 2^-4 / sqrt(3) of a
+    # value in the mean, at some of seven products a layer
+    assert _norm_off(got["out"], out.detach()) < 0.1
+    assert _norm_off(got["grad"], model.layers[0].mlp.down_proj.weight.grad[:, :256]) < 0.3
