@@ -17,13 +17,13 @@
 // DEEP: a tile's contraction is several sums (kDeepestSum says why), each in the accumulator whose turn it is; the
 // epilogue adds them in 128 registers a thread, while the next one is in the making. For these the registers of the other
 // warps go to those of the epilogue, so warpgroups have one role each: warps 4-7 scales, 8-15 epilogue. The gradient of
-// gate and up at 4097 x 2048 x 8192 then is off fp32 sums' by 1.4e-4 of its norm for 1.7e-4, gate and up round on another
+// gate and up at 4097 x 2048 x 8192 then is off fp32 sums' by 1.45e-4 of its norm for 1.66e-4, gate and up round on another
 // side than in 64 bits in 4e-5 of the values for 7e-5 (8192 deep: 1.4e-4 for 3.2e-4). Measured in turn without / with,
 // training steps: 4097 x 2048 x 8192 798 / 817 us, 16384 x 2560 x 9728 3754 / 3881.
 //
-// Measured by itself, L2 flushed: 8192 x 4096 x 4096 92 us (2.98 PFLOP/s, the tensor pipe active in 81 % of the cycles),
-// 20960 x 6144 x 4096 334 us (3.16; 360 inside the layer), 16384 x 4096 x 4096 168 (3.27). Bound by the tensor cores where
-// the contraction is deep, and by the power limit over seconds; by the epilogue where it is short (8192 x 8192 x 512 45 us).
+// Measured by itself, L2 flushed: 8192 x 4096 x 4096 93 us (2.97 PFLOP/s, the tensor pipe active in 81 % of the cycles),
+// 20960 x 6144 x 4096 338 us (3.12; 352 inside the layer), 16384 x 4096 x 4096 172 (3.20). Bound by the tensor cores where
+// the contraction is deep, and by the power limit over seconds; by the epilogue where it is short (8192 x 8192 x 512 47 us).
 // Rows stored from registers, for staging them in shared memory: 95.6 -> 92.9 us under the profiler at the first size.
 #include <cuda_bf16.h>
 

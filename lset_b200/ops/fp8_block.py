@@ -639,7 +639,9 @@ def gated_mlp_fp8_block(x: torch.Tensor, w_gate, w_up, w_down, kind: str = "swig
     ``quantize_fp8_block(w, tile=True)`` gives, all of them, with a fused gate and up weight.
 
     Gate and up products, ``act(gate) * up`` and its gradient, and the gradients of gate and up are rounded to
-    bf16, as they are between separate layers, before they are cast; so are ``y`` and ``dx``, whatever ``x``'s type.
+    bf16, as they are between separate layers, before they are cast; so are ``y`` and ``dx``, whatever ``x``'s type. A
+    training step adds gate, up and dh from parts 1024 deep (an error in them can move a gradient by a step of 8
+    bits); with kept weights they are summed whole, and above ``H`` = 1024 may differ from a step's in the last bit.
     """
     if kind not in _KINDS:
         raise ValueError(f"unknown activation {kind!r}; choose from {tuple(_KINDS)}")
